@@ -132,6 +132,42 @@ def rope_and_cache(
     ref.reshape_and_cache(k, v, k_cache, v_cache, slot_mapping)
 
 
+def qk_norm_rope_and_cache(
+    q: torch.Tensor,             # [T, Hq, D] bf16, any strides of rows and heads
+    k: torch.Tensor,             # [T, Hk, D]
+    v: torch.Tensor,             # [T, Hk, D]
+    q_weight: torch.Tensor,      # [D] bf16
+    k_weight: torch.Tensor,      # [D]
+    eps: float,
+    k_cache: torch.Tensor,       # [NB, Hk, BS, D] bf16 | fp8_e4m3fn
+    v_cache: torch.Tensor,       # [NB, Hk, D, BS]
+    positions: torch.Tensor,     # [T]
+    cos_sin: torch.Tensor,       # [positions, rot] fp32, rot <= D
+    slot_mapping: torch.Tensor,  # [T]
+    is_neox: bool = True,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> torch.Tensor:
+    """Every query and key head RMS-normed and its first rot values rotated (halves, or
+    neighbouring pairs where is_neox is false) in fp32, rounded once: queries are
+    returned as rows [T, Hq, D], keys and values appended to the paged cache, an fp8
+    cache holding them over its scale, clamped to its range. q, k and v stay as they
+    are. One launch in place of the copies, norms and rope_and_cache().
+
+    A slot below 0 or past the cache stores nothing (rows that pad a batch); a position
+    outside the table makes NaN; two rows of one slot leave either's values. There is no
+    gradient: inputs that require one are refused."""
+    positions = positions.to(torch.int32)
+    slot_mapping = slot_mapping.to(torch.int64)
+    if q.is_cuda:
+        return _require_ext("qk_norm_rope_and_cache").qk_norm_rope_and_cache(
+            q, k, v, q_weight, k_weight, eps, k_cache, v_cache, positions, cos_sin,
+            slot_mapping, is_neox, k_scale, v_scale)
+    return ref.qk_norm_rope_and_cache(q, k, v, q_weight, k_weight, eps, k_cache, v_cache,
+                                      positions, cos_sin, slot_mapping, is_neox, k_scale,
+                                      v_scale)
+
+
 def reshape_and_cache(
     k: torch.Tensor,
     v: torch.Tensor,
@@ -244,6 +280,43 @@ def paged_attention_decode(
     return ref.paged_attention_decode(
         q, k_cache, v_cache, block_tables, seq_lens, scale, sliding_window, softcap, sinks
     )
+
+
+def shared_prefix_attention_decode(
+    q: torch.Tensor,             # [B, Hq, D] bf16 (rows may be strided)
+    k_cache: torch.Tensor,       # [NB, Hk, BS, D] bf16 | fp8_e4m3fn
+    v_cache: torch.Tensor,       # [NB, Hk, D, BS]
+    block_tables: torch.Tensor,  # [B, max_blocks]
+    seq_lens: torch.Tensor,      # [B]
+    prefix_group: torch.Tensor,  # [B] the group of each row, -1: none
+    prefix_lens: torch.Tensor,   # [N] tokens that a group's rows share
+    scale: float,
+    sliding_window: int = -1,
+    softcap: float = 0.0,
+    sinks: Optional[torch.Tensor] = None,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> torch.Tensor:
+    """paged_attention_decode() of rows that share prefixes, whose keys and values are
+    read once for all rows of a group: the first prefix_lens[g] tokens of every row of
+    group g are read through the block table of the first of them, the rest through the
+    row's own. A prefix need not end with a page. A row shorter than its group's prefix
+    counts as one without a group, and so does one of a group outside of prefix_lens; a
+    row of length 0 gives zeros. Lengths and groups are read on the device only, so that
+    a captured call follows them. Pages outside the cache are read as its nearest one.
+    There is no gradient: a q that requires one is refused."""
+    block_tables, seq_lens, prefix_group, prefix_lens = (
+        t.to(torch.int32) for t in (block_tables, seq_lens, prefix_group, prefix_lens))
+    if sinks is not None:
+        sinks = sinks.float()
+    if q.is_cuda:
+        return _require_ext(
+            "shared_prefix_attention_decode").shared_prefix_attention_decode(
+                q, k_cache, v_cache, block_tables, seq_lens, prefix_group, prefix_lens,
+                scale, sliding_window, softcap, sinks, k_scale, v_scale)
+    return ref.shared_prefix_attention_decode(
+        q, k_cache, v_cache, block_tables, seq_lens, prefix_group, prefix_lens, scale,
+        sliding_window, softcap, sinks, k_scale, v_scale)
 
 
 def rope_cache_attention_decode(

@@ -1435,7 +1435,19 @@ torch::Tensor lt_linear(torch::Tensor x, torch::Tensor w);  // lt_gemm.cpp
 torch::Tensor lt_linear_fp8(torch::Tensor x_q, torch::Tensor w_q,
                             torch::Tensor x_scale, torch::Tensor w_scale);
 
+// cache_ops.cpp
+torch::Tensor qk_norm_rope_and_cache(torch::Tensor, torch::Tensor, torch::Tensor,
+                                     torch::Tensor, torch::Tensor, double,
+                                     torch::Tensor, torch::Tensor, torch::Tensor,
+                                     torch::Tensor, torch::Tensor, bool, double, double);
+torch::Tensor shared_prefix_attention_decode(torch::Tensor, torch::Tensor, torch::Tensor,
+                                             torch::Tensor, torch::Tensor, torch::Tensor,
+                                             torch::Tensor, double, int64_t, double,
+                                             std::optional<torch::Tensor>, double, double);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("qk_norm_rope_and_cache", &qk_norm_rope_and_cache);
+  m.def("shared_prefix_attention_decode", &shared_prefix_attention_decode);
   m.def("lt_linear_fp8", &lt_linear_fp8,
         "fp8-E4M3 W8A8 y = (xq*sx) @ (wq*sw)^T (bf16 out)");
   m.def("lt_linear", &lt_linear,

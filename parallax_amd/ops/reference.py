@@ -111,6 +111,58 @@ def reshape_and_cache(
     v_cache[blk, :, :, off] = v[valid].to(v_cache.dtype)
 
 
+def qk_norm_rope_and_cache(
+    q: torch.Tensor,             # [T, Hq, D]
+    k: torch.Tensor,             # [T, Hk, D]
+    v: torch.Tensor,             # [T, Hk, D]
+    q_weight: torch.Tensor,      # [D]
+    k_weight: torch.Tensor,      # [D]
+    eps: float,
+    k_cache: torch.Tensor,       # [num_blocks, Hk, block_size, D]
+    v_cache: torch.Tensor,       # [num_blocks, Hk, D, block_size]
+    positions: torch.Tensor,     # [T] int
+    cos_sin: torch.Tensor,       # [P, rot_dim] fp32
+    slot_mapping: torch.Tensor,  # [T] int; outside the cache: nothing is stored
+    is_neox: bool = True,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> torch.Tensor:
+    T, _, D = q.shape
+    rot, P = cos_sin.shape[-1], cos_sin.shape[0]
+    if rot % 2 or rot > D or k.shape != v.shape or k.shape[0] != T or k.shape[2] != D:
+        raise RuntimeError("q, k, v and cos_sin do not fit each other")
+    if torch.is_grad_enabled() and any(
+            t.requires_grad for t in (q, k, v, q_weight, k_weight)):
+        raise RuntimeError("there is no gradient: call it under no_grad")
+    known = (positions >= 0) & (positions < P)
+    cs = cos_sin[positions.long().clamp(0, max(P - 1, 0))].masked_fill(
+        ~known.unsqueeze(-1), float("nan")).unsqueeze(1)
+    cos, sin = cs[..., : rot // 2], cs[..., rot // 2:]
+    one = slice(0, rot // 2) if is_neox else slice(0, rot, 2)
+    two = slice(rot // 2, rot) if is_neox else slice(1, rot, 2)
+
+    def turn(x, w):
+        y = x.float()
+        y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+        z = y.clone()
+        z[..., one] = y[..., one] * cos - y[..., two] * sin
+        z[..., two] = y[..., two] * cos + y[..., one] * sin
+        return z
+
+    def held(x, cache, scale):
+        if cache.dtype == torch.float8_e4m3fn:
+            x = (x / scale).clamp(-448.0, 448.0)
+        return x.to(cache.dtype)
+
+    block_size = k_cache.shape[2]
+    valid = (slot_mapping >= 0) & (slot_mapping < k_cache.shape[0] * block_size)
+    slots = slot_mapping[valid].long()
+    blk, off = slots // block_size, slots % block_size
+    k_cache[blk, :, off] = held(turn(k, k_weight)[valid], k_cache, k_scale)
+    v_cache[blk, :, :, off] = held(v.float()[valid], v_cache, v_scale)
+    return turn(q, q_weight).to(q.dtype)
+
+
 def mla_reshape_and_cache(
     kv_latent: torch.Tensor,     # [T, lora_rank]
     k_rope: torch.Tensor,        # [T, rope_dim]
@@ -179,6 +231,52 @@ def paged_attention_decode(
         if sinks is not None:
             p = p[:, 1:]
         out[i] = torch.einsum("hl,hld->hd", p, vf).to(q.dtype)
+    return out
+
+
+def shared_prefix_attention_decode(
+    q: torch.Tensor,             # [B, Hq, D]
+    k_cache: torch.Tensor,       # [num_blocks, Hk, bs, D]
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,  # [B, max_blocks] int
+    seq_lens: torch.Tensor,      # [B] int
+    prefix_group: torch.Tensor,  # [B] int, -1: no group
+    prefix_lens: torch.Tensor,   # [N] int
+    scale: float,
+    sliding_window: int = -1,
+    softcap: float = 0.0,
+    sinks: Optional[torch.Tensor] = None,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> torch.Tensor:
+    """A row's tokens before its group's prefix through the pages of the group's first
+    row, the others through its own."""
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise RuntimeError("there is no gradient: call it under no_grad")
+    B, Hq, D = q.shape
+    Hk, block_size = k_cache.shape[1:3]
+    out = torch.zeros_like(q)
+    first = {}
+    lens, prefix = seq_lens.tolist(), prefix_lens.tolist()
+    for b, (L, g) in enumerate(zip(lens, prefix_group.tolist())):
+        P = prefix[g] if 0 <= g < len(prefix) and 0 < prefix[g] <= L else 0
+        if L <= 0:
+            continue
+        owner = first.setdefault(g, b) if P else b
+        tok = torch.arange(max(0, L - sliding_window) if sliding_window > 0 else 0, L,
+                           device=q.device)
+        row = torch.where(tok < P, owner, b)
+        page = block_tables[row, tok // block_size].long().clamp(0, k_cache.shape[0] - 1)
+        k = k_cache[page, :, tok % block_size].float() * k_scale     # [L, Hk, D]
+        v = v_cache[page, :, :, tok % block_size].float() * v_scale
+        x = q[b].float().view(Hk, Hq // Hk, D)
+        z = torch.einsum("hgd,lhd->hgl", x, k).reshape(Hq, -1) * scale
+        if softcap > 0:
+            z = softcap * torch.tanh(z / softcap)
+        if sinks is not None:
+            z = torch.cat([z, sinks.float().unsqueeze(-1)], dim=-1)
+        p = torch.softmax(z, dim=-1)[:, : len(tok)].view(Hk, Hq // Hk, -1)
+        out[b] = torch.einsum("hgl,lhd->hgd", p, v).reshape(Hq, D).to(q.dtype)
     return out
 
 

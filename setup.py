@@ -2,8 +2,8 @@
 
     PYTORCH_ROCM_ARCH=gfx950 python setup.py build_ext --inplace
 
-The built .so files land at parallax_amd/ops/_C.*.so (attention, GEMM, MoE,
-sampler kernels) and parallax_amd/ops/_mix.*.so (sequence mixers: fp32-residual
+The built .so files land at parallax_amd/ops/_C.*.so (attention, cache, GEMM,
+MoE, sampler kernels) and parallax_amd/ops/_mix.*.so (sequence mixers: fp32-residual
 layer norm, sliding-window latent attention, gated linear attention, sandwich
 RMS norm, row-cache attention, post-norm residual step, minGRU, hyper-connected
 streams, matrix LSTM, softmax router, fixed-decay linear attention, gated delta
@@ -25,10 +25,13 @@ CSRC = os.path.join(ROOT, "parallax_amd", "ops", "csrc")
 sources = [
     os.path.join(CSRC, "bindings.cpp"),
     os.path.join(CSRC, "lt_gemm.cpp"),
+    os.path.join(CSRC, "cache_ops.cpp"),
     os.path.join(CSRC, "elementwise.hip"),
     os.path.join(CSRC, "paged_attention.hip"),
     os.path.join(CSRC, "paged_attention_mfma.hip"),
     os.path.join(CSRC, "paged_decode.hip"),
+    os.path.join(CSRC, "shared_prefix.hip"),
+    os.path.join(CSRC, "head_norm_store.hip"),
     os.path.join(CSRC, "mla_attention.hip"),
     os.path.join(CSRC, "mla_prefill.hip"),
     os.path.join(CSRC, "prefill_attention.hip"),
