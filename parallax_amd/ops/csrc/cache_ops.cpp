@@ -16,6 +16,7 @@
 #include <cmath>
 #include <initializer_list>
 #include <optional>
+#include <utility>
 
 struct HeadNormStore {
   uint16_t* out;
@@ -40,10 +41,16 @@ struct SharedPrefix {
   int64_t q_stride;
   float scale, v_scale, softcap;
   int window;
+  int p_runs, s_runs;
+  float *p_acc, *p_ml;
+  int4* p_info;
+  float *s_acc, *s_ml;
+  int2* s_info;
 };
 
 extern "C" {
 void launch_head_norm_store(const HeadNormStore*, bool, bool, hipStream_t);
+void shared_prefix_plan(int, int, int, int, int, int*, int*, int*);
 void launch_shared_prefix(const SharedPrefix*, bool, hipStream_t);
 }
 
@@ -101,6 +108,8 @@ float scale_of(double s, const char* name) {
   TORCH_CHECK(std::isfinite(s) && s > 0, name, " must be above 0");
   return (float)s;
 }
+
+Tensor from16(const Tensor& t) { return (uintptr_t)t.data_ptr() % 16 ? t.clone() : t; }
 
 hipStream_t stream() { return at::hip::getCurrentHIPStream().stream(); }
 
@@ -189,7 +198,14 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   TORCH_CHECK(prefix_lens.dim() == 1, "prefix_lens must be a list");
   const int64_t N = prefix_lens.size(0);
   check_list(prefix_lens, at::kInt, N, "prefix_lens");
-  TORCH_CHECK(B <= 4096 && N <= 4096, "at most 4096 rows and groups");
+  TORCH_CHECK(B <= 4096 && N <= 256, "at most 4096 rows and 256 groups");
+  const int64_t max_blocks = block_tables.size(1);
+  // key tiles of all item tiles, and units of all rows, are counted in 32 bits
+  TORCH_CHECK(max_blocks * BS < INT_MAX / 4 &&
+                  (B * Hq / Hk / 128 + N) * (max_blocks * BS / 64 + 1) < INT_MAX &&
+                  B * (max_blocks * BS / 128 + 1) < INT_MAX &&
+                  Hk * BS * D <= INT_MAX && Hq <= 65535,
+              "too many tokens or heads");
   TORCH_CHECK(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0,
               "scale and softcap must be finite, softcap not negative");
   if (sinks) check_list(*sinks, at::kFloat, Hq, "sinks");
@@ -202,7 +218,11 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   const c10::DeviceGuard guard(q.device());
   auto out = torch::empty({B, Hq, D}, q.options());
   if (B == 0) return out;
-  if (block_tables.size(1) == 0 || k_cache.size(0) == 0) return out.zero_();
+  // copied to LDS and read by 16 bytes at once
+  k_cache = from16(k_cache);
+  v_cache = from16(v_cache);
+  if ((uintptr_t)q.data_ptr() % 16 || q.stride(0) % 8) q = q.clone(at::MemoryFormat::Contiguous);
+  if (max_blocks == 0 || k_cache.size(0) == 0) return out.zero_();
   const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
   SharedPrefix a = {};
   a.out = (uint16_t*)out.data_ptr();
@@ -216,12 +236,28 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   a.sinks = sinks ? sinks->data_ptr<float>() : nullptr;
   a.B = B, a.N = N, a.Hq = Hq, a.Hk = Hk, a.D = D;
   a.shift = BS == 16 ? 4 : BS == 32 ? 5 : 6;
-  a.max_blocks = block_tables.size(1), a.num_pages = k_cache.size(0);
+  a.max_blocks = max_blocks, a.num_pages = k_cache.size(0);
   a.q_stride = q.stride(0);
   a.scale = (float)(fp8 ? scale * k_scale : scale);
   a.v_scale = fp8 ? (float)v_scale : 1.f;
   a.softcap = (float)softcap;
   a.window = sliding_window > 0 ? (int)std::min<int64_t>(sliding_window, INT_MAX) : 0;
+  int tiles;
+  shared_prefix_plan(a.B, a.N, a.Hq, a.Hk, a.D, &a.p_runs, &a.s_runs, &tiles);
+  // fp32 words: of a part its sums, then maxima and sums of weights; then where a row's
+  // parts lie
+  const int64_t p_items = N > 0 ? (int64_t)(a.p_runs + tiles) * Hk * 128 : 0;
+  const int64_t s_items = (a.s_runs + B) * Hq;
+  const int64_t words = (p_items + s_items) * (D + 2) + B * Hq * 4 + B * 2;
+  auto work = torch::empty({words}, q.options().dtype(at::kFloat));
+  float* at = work.data_ptr<float>();
+  auto take = [&](int64_t n) { return std::exchange(at, at + n); };
+  a.p_acc = take(p_items * D);
+  a.s_acc = take(s_items * D);
+  a.p_info = (int4*)take(B * Hq * 4);
+  a.p_ml = take(p_items * 2);
+  a.s_ml = take(s_items * 2);
+  a.s_info = (int2*)take(B * 2);
   launch_shared_prefix(&a, fp8, stream());
   return out;
 }

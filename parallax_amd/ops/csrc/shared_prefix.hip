@@ -5,9 +5,40 @@
 // Row b belongs to group g = prefix_group[b] if 0 <= g < N and its length is at least
 // prefix_lens[g] > 0; its tokens before prefix_lens[g] are then those of the pages of
 // the group's first row, the others those of its own. All other rows have no group.
+//
+// One launch has two kinds of workgroups, whose parts (a maximum, a sum of weights and
+// a sum of weighted values, in fp32) a second launch joins:
+//
+// Prefixes. The (row, query head) items of a group and key/value head are columns, 128
+// a tile, 32 a wave; keys go by in tiles of 64 that all of them read:
+//   S^T[64 x 32] = K . Q^T    O^T[D x 32] += V^T . P     mfma_f32_32x32x16_bf16
+// K rows are taken with bits 2 and 3 of their number swapped, so that an accumulator
+// half of S^T is eight neighbouring tokens, the operand of the second product: P stays
+// in registers. The key tiles of all item tiles of all groups form one list, of which
+// every workgroup takes an equal run.
+//
+// Suffixes. The tokens behind the prefix (of a row without a group: all) are decode
+// attention as in paged_decode.hip: a wave copies tiles of 32 tokens into LDS of its
+// own, a key/value head's query heads are 16 columns; units of 128 tokens of all rows
+// form one list, dealt in equal runs.
+//
+// Lengths, groups and prefixes are read on the device, by every workgroup itself; the
+// grid depends on sizes alone.
+
+#include <algorithm>
+#include <climits>
 
 #include "common.h"
 #include "decode_common.h"
+#include "decode_tiles.h"
+
+#define SP_KT 64       // keys of a prefix tile
+#define SP_ITEMS 128   // items of one
+#define SP_UNIT 128    // tokens of a suffix unit: 32 a wave
+#define SP_GROUPS 256  // at most
+#define SP_ROWS 4096   // at most
+
+typedef float f32x16v __attribute__((ext_vector_type(16)));
 
 struct SharedPrefix {
   uint16_t* out;           // [B, Hq, D]
@@ -19,11 +50,17 @@ struct SharedPrefix {
   int64_t q_stride;
   float scale, v_scale, softcap;  // scale: with that of an fp8 cache's keys
   int window;
+  // workgroups of a key/value head: for prefixes, for suffixes
+  int p_runs, s_runs;
+  float* p_acc;  // [p_parts, Hk, SP_ITEMS, D]: part run + item tile
+  float* p_ml;   // [p_parts, Hk, SP_ITEMS, 2] maxima in units of log2, sums
+  int4* p_info;  // [B, Hq]: first part, parts, place in them; rows of a group only
+  float* s_acc;  // [s_runs + B, Hq, D]: part run + row
+  float* s_ml;   // [s_runs + B, Hq, 2]
+  int2* s_info;  // [B]: first and last run; rows with tokens behind a prefix only
 };
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 DEVINL int prefix_of(const SharedPrefix& a, int b) {
   const int g = a.group[b];
@@ -31,64 +68,778 @@ DEVINL int prefix_of(const SharedPrefix& a, int b) {
   return p > 0 && a.lens[b] >= p ? p : 0;
 }
 
-}  // namespace
+DEVINL int window_start(const SharedPrefix& a, int L) {
+  return a.window > 0 ? max(0, L - a.window) : 0;
+}
 
-template <bool FP8>
-__global__ __launch_bounds__(64) void shared_prefix_kernel(const SharedPrefix a) {
-  __shared__ float qs[128];
-  const int lane = threadIdx.x, h = blockIdx.x, b = blockIdx.y;
-  const int hk = h / (a.Hq / a.Hk), BS = 1 << a.shift, D = a.D;
-  const int L = a.lens[b], P = prefix_of(a, b);
-  const int lo = a.window > 0 ? max(0, L - a.window) : 0;
-  int first = b;
-  if (P > 0)
-    for (int i = b - 1; i >= 0; --i)
-      if (a.group[i] == a.group[b] && prefix_of(a, i) > 0) first = i;
-  for (int d = lane; d < D; d += 64)
-    qs[d] = bf16_bits_to_f32(a.q[b * a.q_stride + h * D + d]);
+// units of a row's tokens [lo, L)
+DEVINL int suffix_units(int lo, int L) {
+  return L > lo ? (L + SP_UNIT - 1) / SP_UNIT - lo / SP_UNIT : 0;
+}
+
+DEVINL int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+DEVINL int page_at(const SharedPrefix& a, int entry) {
+  return min(max(entry, 0), a.num_pages - 1);
+}
+
+template <class F>
+DEVINL float over_halves(float v, F f) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v),
+                                                  __float_as_uint(v), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+constexpr int tiles_bytes(int D) { return 4 * SP_KT * D * 2; }
+constexpr int lds_bytes(int D) {
+  return tiles_bytes(D) + (2 * SP_GROUPS + SP_ITEMS + 4) * 4 + SP_ROWS * 2;
+}
+
+// ---- prefixes ----------------------------------------------------------------------
+
+template <int D, bool FP8>
+DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const int run) {
+  constexpr int KCH = D / 8;            // 16-byte chunks of a K row
+  constexpr int KPER = SP_KT * KCH / 256;  // chunks that a thread copies
+  constexpr int VPER = D * 8 / 256;
+  constexpr int KSTEPS = D / 16;
+  constexpr int DT = D / 32;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wid = uniform(tid >> 6);
+  const int half = lane >> 5;
+  const int l31 = lane & 31;
+  const int G = a.Hq / a.Hk, BS = 1 << a.shift;
+
+  uint16_t* const K0 = (uint16_t*)S;
+  uint16_t* const V0 = K0 + SP_KT * D;
+  uint16_t* const K1 = V0 + SP_KT * D;
+  uint16_t* const V1 = K1 + SP_KT * D;
+  int* const count = (int*)(S + tiles_bytes(D));  // rows of a group
+  int* const low = count + SP_GROUPS;             // where the first window begins
+  int* const rows = low + SP_GROUPS;              // of an item tile; 130: the group's first
+  int16_t* const member = (int16_t*)(rows + SP_ITEMS + 4);  // a row's group
+
+  for (int g = tid; g < a.N; g += 256) {
+    count[g] = 0;
+    low[g] = INT_MAX;
+  }
   __syncthreads();
-  float m = -1e30f, l = 0.f, o[2] = {};
-  for (int t0 = lo; t0 < L; t0 += 64) {
-    const int tok = t0 + lane;
-    const bool on = tok < L;
-    const int at = min(tok, L - 1);
-    const int* table = a.tables + (int64_t)(at < P ? first : b) * a.max_blocks;
-    const int page = min(max(table[at >> a.shift], 0), a.num_pages - 1);
-    const int64_t row = (int64_t)page * a.Hk + hk;
-    const int64_t k0 = (row * BS + (at & (BS - 1))) * D;
-    float s = 0.f;
-    for (int d = 0; d < D; ++d)
-      s = fmaf(FP8 ? fp8_e4m3_to_f32(a.k[k0 + d])
-                   : bf16_bits_to_f32(((const uint16_t*)a.k)[k0 + d]), qs[d], s);
-    s *= a.scale;
-    if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
-    s = on ? s * kLog2e : -__builtin_inff();
-    const float m2 = fmaxf(m, wave_reduce_max(s));
-    const float f = exp2f(m - m2), p = exp2f(s - m2);
-    m = m2;
-    l = l * f + p;
-    o[0] *= f;
-    o[1] *= f;
-    for (int j = 0; j < 64 && t0 + j < L; ++j) {
-      const float w = __shfl(p, j, WAVE_SIZE);
-      const int64_t r = (int64_t)__shfl(page, j, WAVE_SIZE) * a.Hk + hk;
-      for (int i = 0; i < D / 64; ++i) {
-        const int64_t v0 = (r * D + i * 64 + lane) * BS + ((t0 + j) & (BS - 1));
-        o[i] = fmaf(w, FP8 ? fp8_e4m3_to_f32(a.v[v0])
-                           : bf16_bits_to_f32(((const uint16_t*)a.v)[v0]), o[i]);
-      }
+  for (int b = tid; b < a.B; b += 256) {
+    const int p = prefix_of(a, b);
+    const int g = p > 0 ? a.group[b] : -1;
+    member[b] = (int16_t)g;
+    if (g >= 0) {
+      atomicAdd(count + g, 1);
+      atomicMin(low + g, window_start(a, a.lens[b]));
     }
   }
-  l = wave_reduce_sum(l);
-  if (a.sinks != nullptr) l += exp2f(a.sinks[h] * kLog2e - m);
-  const float inv = L > 0 ? a.v_scale / l : 0.f;
-  for (int i = 0; i < D / 64; ++i)
-    a.out[((int64_t)b * a.Hq + h) * D + i * 64 + lane] =
-        (uint16_t)pack_bf16(o[i] * inv, 0.f);
+  __syncthreads();
+
+  // ---- this workgroup's run of key tiles ------------------------------------------
+  auto tiles_of = [&](int g) { return (count[g] * G + SP_ITEMS - 1) / SP_ITEMS; };
+  auto keys_of = [&](int g, int* begin) {  // at least one tile
+    const int end = (a.prefix[g] + SP_KT - 1) / SP_KT;
+    *begin = min(low[g] / SP_KT, end - 1);
+    return end;
+  };
+  int g = 0, at = 0, tile0 = 0, todo = 0, per = 1, begin = 0;
+  {
+    int total = 0;
+    for (int g0 = 0; g0 < a.N; g0 += 64) {
+      const int x = g0 + lane;
+      int kb, n = 0;
+      if (x < a.N && count[x] > 0) n = tiles_of(x) * (keys_of(x, &kb) - kb);
+      total += __shfl(scan64(n), 63, WAVE_SIZE);
+    }
+    per = max((total + a.p_runs - 1) / a.p_runs, 1);
+    begin = run * per;
+    if (begin >= total) return;
+    todo = min(per, total - begin);
+    int before = 0;
+    for (int g0 = 0; g0 < a.N; g0 += 64) {
+      const int x = g0 + lane;
+      int kb, n = 0, t = 0;
+      if (x < a.N && count[x] > 0) {
+        t = tiles_of(x);
+        n = t * (keys_of(x, &kb) - kb);
+      }
+      const int ns = scan64(n), ts = scan64(t);
+      const unsigned long long hit = __ballot(before + ns > begin);
+      if (hit) {
+        const int src = __ffsll(hit) - 1;
+        g = g0 + src;
+        at = begin - before - __shfl(ns, src, WAVE_SIZE) + __shfl(n, src, WAVE_SIZE);
+        tile0 += __shfl(ts, src, WAVE_SIZE) - __shfl(t, src, WAVE_SIZE);
+        break;
+      }
+      before += __shfl(ns, 63, WAVE_SIZE);
+      tile0 += __shfl(ts, 63, WAVE_SIZE);
+    }
+  }
+  g = uniform(g);
+  at = uniform(at);
+  tile0 = uniform(tile0);
+  todo = uniform(todo);
+  per = uniform(per);
+  begin = uniform(begin);
+
+  // ---- what a lane copies and reads -------------------------------------------------
+  // 16 chunks (256 bytes) make a turn over the banks: a K row of 128 values, or two of
+  // 64; a V row has 64 tokens, so two as well
+  auto k_swz = [](int r) INL { return D == 128 ? r & 15 : (r >> 1) & 7; };
+  auto k_row = [&](int i) INL { return ((wid * KPER + i) * 64 + lane) / KCH; };
+  auto v_row = [&](int i) INL { return (wid * VPER + i) * 8 + (lane >> 3); };
+  auto v_src = [&](int i) INL { return (lane & 7) ^ ((v_row(i) >> 1) & 7); };
+  const uint32_t page_elems = (uint32_t)a.Hk * BS * D;
+  int koff[KPER], voff[VPER];
+#pragma unroll
+  for (int i = 0; i < KPER; ++i)
+    koff[i] = (hk * BS + (k_row(i) & (BS - 1))) * D + ((lane % KCH) ^ k_swz(k_row(i))) * 8;
+#pragma unroll
+  for (int i = 0; i < VPER; ++i)
+    voff[i] = (hk * D + v_row(i)) * BS + ((v_src(i) * 8) & (BS - 1));
+  const int krow = (l31 & 0x13) | ((l31 & 4) << 1) | ((l31 & 8) >> 1);
+  auto k_frag = [&](const uint16_t* Kl, int ks, int t) INL {
+    const int pos = (2 * ks + half) ^ k_swz(krow);
+    return *reinterpret_cast<const bf16x8v*>(Kl + (t * 32 + krow) * D + pos * 8);
+  };
+  auto v_frag = [&](const uint16_t* Vl, int ks, int t) INL {
+    const int d = t * 32 + l31;
+    const int pos = (2 * ks + half) ^ ((d >> 1) & 7);
+    return *reinterpret_cast<const bf16x8v*>(Vl + d * SP_KT + pos * 8);
+  };
+  // above 0 also for a scale of 0: hidden scores are multiplied by it too
+  const float c = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1e-20f);
+
+  int done = 0;
+  while (todo > 0) {
+    const int n_items = count[g] * G;
+    const int P = a.prefix[g];
+    int kb;
+    const int kend = uniform(keys_of(g, &kb));
+    kb = uniform(kb);
+    const int keys = kend - kb;
+    const int tile = at / keys;
+    const int k0 = kb + at % keys, k1 = min(kend, k0 + todo);
+
+    // ---- the tile's items ---------------------------------------------------------
+    const int r0 = tile * SP_ITEMS / G;
+    const int r1 = (min((tile + 1) * SP_ITEMS, n_items) - 1) / G;
+    __syncthreads();  // the buffers and the list are free
+    if (wid == 0) {
+      int rank = 0;
+      for (int b0 = 0; b0 < a.B && rank <= r1; b0 += 64) {
+        const bool is = b0 + lane < a.B && member[b0 + lane] == g;
+        const unsigned long long all = __ballot(is);
+        const int mine = rank + __popcll(all & ((1ull << lane) - 1));
+        if (is && mine >= r0 && mine <= r1) rows[mine - r0] = b0 + lane;
+        if (is && mine == 0) rows[SP_ITEMS + 2] = b0 + lane;
+        rank += __popcll(all);
+      }
+    }
+    __syncthreads();
+    const int item = tile * SP_ITEMS + wid * 32 + l31;
+    const bool on = item < n_items;
+    const int r = min(item, n_items - 1) / G;
+    const int row = rows[r - r0];
+    const int h = hk * G + min(item, n_items - 1) - r * G;
+    const int lo = window_start(a, a.lens[row]);
+    // constant memory: read by the scalar unit
+    const auto* table = (const __attribute__((address_space(4))) int*)(
+        a.tables + (size_t)uniform(rows[SP_ITEMS + 2]) * a.max_blocks);
+    const bool wave_on = tile * SP_ITEMS + wid * 32 < n_items;
+    int lo_most = lo;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+      lo_most = max(lo_most, __shfl_xor(lo_most, o, WAVE_SIZE));
+    lo_most = uniform(lo_most);
+    const int lo_least = low[g];
+
+    if (k0 == kb && half == 0 && on)
+      a.p_info[(int64_t)row * a.Hq + h] =
+          make_int4(run + tile0 + tile, (begin + done + keys - 1) / per - run + 1,
+                    item - tile * SP_ITEMS, 0);
+
+    bf16x8v qf[KSTEPS];
+    {
+      const uint16_t* src = a.q + row * a.q_stride + h * D + half * 8;
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s) {
+        u32x4v x = *reinterpret_cast<const u32x4v*>(src + s * 16);
+        if (a.scale < 0.f) x ^= 0x80008000u;  // the sign goes with q
+        qf[s] = __builtin_bit_cast(bf16x8v, x);
+      }
+    }
+
+    int kpage = 0, vpage[2] = {0, 0};
+    auto pages = [&](int kt) INL {  // of the rows and chunks that this thread copies
+      kpage = page_at(a, table[min(kt * SP_KT + wid * 16, P - 1) >> a.shift]);
+      const int* t = (const int*)table;
+      vpage[0] = page_at(a, t[min(kt * SP_KT + v_src(0) * 8, P - 1) >> a.shift]);
+      vpage[1] = page_at(a, t[min(kt * SP_KT + v_src(1) * 8, P - 1) >> a.shift]);
+    };
+    auto k_elem = [&](int i) INL {
+      return (uint64_t)(uint32_t)kpage * page_elems + (uint32_t)koff[i];
+    };
+    auto v_elem = [&](int i) INL {
+      return (uint64_t)(uint32_t)vpage[i & 1] * page_elems + (uint32_t)voff[i];
+    };
+    uint64_t kraw[FP8 ? KPER : 1], vraw[FP8 ? VPER : 1];
+    auto issue = [&](uint16_t* Kl, uint16_t* Vl) INL {
+      if constexpr (FP8) {
+#pragma unroll
+        for (int i = 0; i < KPER; ++i)
+          kraw[i] = *reinterpret_cast<const uint64_t*>(a.k + k_elem(i));
+#pragma unroll
+        for (int i = 0; i < VPER; ++i)
+          vraw[i] = *reinterpret_cast<const uint64_t*>(a.v + v_elem(i));
+      } else {
+#pragma unroll
+        for (int i = 0; i < KPER; ++i)
+          copy16_to_lds((const uint16_t*)a.k + k_elem(i), Kl + (wid * KPER + i) * 512);
+#pragma unroll
+        for (int i = 0; i < VPER; ++i)
+          copy16_to_lds((const uint16_t*)a.v + v_elem(i), Vl + (wid * VPER + i) * 512);
+      }
+    };
+    auto settle = [&](uint16_t* Kl, uint16_t* Vl) INL {  // fp8: what was asked for
+      if constexpr (FP8) {
+#pragma unroll
+        for (int i = 0; i < KPER; ++i)
+          *reinterpret_cast<bf16x8v*>(Kl + ((wid * KPER + i) * 64 + lane) * 8) =
+              widen((uint32_t)kraw[i], (uint32_t)(kraw[i] >> 32));
+#pragma unroll
+        for (int i = 0; i < VPER; ++i)
+          *reinterpret_cast<bf16x8v*>(Vl + ((wid * VPER + i) * 64 + lane) * 8) =
+              widen((uint32_t)vraw[i], (uint32_t)(vraw[i] >> 32));
+      }
+    };
+
+    f32x16v o[DT] = {};
+    float m = kLowest, l = 0.f;
+    auto turn = [&](int kt, const uint16_t* Kl, const uint16_t* Vl, uint16_t* Kn,
+                    uint16_t* Vn) INL {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0x0070);  // all copies, all stores to LDS
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (kt + 1 < k1) {
+        issue(Kn, Vn);
+        pages(min(kt + 2, k1 - 1));
+      }
+      if (wave_on) {
+        const int base = kt * SP_KT;
+        f32x16v s[2] = {};
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(Kl, ks, t), qf[ks],
+                                                           s[t], 0, 0, 0);
+        if (a.softcap > 0.f) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              s[t][e] = a.softcap * tanhf(s[t][e] * fabsf(a.scale) / a.softcap) * kLog2e;
+        }
+        const bool cut = base + SP_KT > P || base < lo_least;
+        if (cut || base < lo_most) {
+          const int end = P - base - 8 * half, first = lo - base - 8 * half;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int tok = 32 * t + 16 * (e >> 3) + (e & 7);
+              s[t][e] = tok < end && tok >= first ? s[t][e] : kHidden;
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
+        mx = over_halves(mx, [](float x, float y) { return fmaxf(x, y); }) * c;
+        // rescaled when a maximum moved: its own weight is then 1, without error
+        if (__any(mx > m)) {
+          const float m2 = fmaxf(m, mx);
+          const float f = __builtin_amdgcn_exp2f(m - m2);
+          m = m2;
+          l *= f;
+#pragma unroll
+          for (int t = 0; t < DT; ++t) o[t] *= f;
+        }
+#pragma unroll
+        for (int ks = 0; ks < SP_KT / 16; ++ks) {
+          u32x4v w;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int e = (ks & 1) * 8 + 2 * j;
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[ks >> 1][e], c, -m));
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[ks >> 1][e + 1], c, -m));
+            l += x;
+            l += y;
+            w[j] = pack_bf16(x, y);
+          }
+          bf16x8v v[DT];
+#pragma unroll
+          for (int t = 0; t < DT; ++t) v[t] = v_frag(Vl, ks, t);
+          if (cut) {  // what no item sees may be anything: weight 0 times it
+            const int end = P - base - 16 * ks - 8 * half;
+            const int first = lo_least - base - 16 * ks - 8 * half;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                v[t][j] = j < end && j >= first ? v[t][j] : (short)0;
+          }
+#pragma unroll
+          for (int t = 0; t < DT; ++t)
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                v[t], __builtin_bit_cast(bf16x8v, w), o[t], 0, 0, 0);
+        }
+      }
+      if (kt + 1 < k1) settle(Kn, Vn);
+    };
+
+    pages(k0);
+    issue(K0, V0);
+    settle(K0, V0);
+    pages(min(k0 + 1, k1 - 1));
+    for (int kt = k0; kt < k1; kt += 2) {
+      turn(kt, K0, V0, K1, V1);
+      if (kt + 1 < k1) turn(kt + 1, K1, V1, K0, V0);
+    }
+
+    l = over_halves(l, [](float x, float y) { return x + y; });
+    if (on) {
+      const int64_t part = ((int64_t)(run + tile0 + tile) * a.Hk + hk) * SP_ITEMS +
+                           item - tile * SP_ITEMS;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4v x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = o[t][4 * i + e];
+          *reinterpret_cast<f32x4v*>(a.p_acc + part * D + t * 32 + 8 * i + 4 * half) = x;
+        }
+      if (half == 0) *reinterpret_cast<f32x2v*>(a.p_ml + part * 2) = f32x2v{m, l};
+    }
+
+    todo -= k1 - k0;
+    done += k1 - k0;
+    at += k1 - k0;
+    const int tiles = tiles_of(g);
+    if (at == tiles * keys) {
+      at = 0;
+      tile0 += tiles;
+      do ++g;
+      while (g < a.N && count[g] == 0);
+      g = uniform(g);
+    }
+  }
+}
+
+// ---- suffixes ----------------------------------------------------------------------
+
+template <int D, bool FP8>
+DEVINL void suffix_role(const SharedPrefix& a, uint8_t* S, const int hk, const int run) {
+  constexpr int W = 4;
+  constexpr int KT = 32;                 // tokens a tile
+  constexpr int ES = FP8 ? 1 : 2;
+  constexpr int RB = D * ES;             // bytes a K row
+  constexpr int CPR = RB / 16;
+  constexpr int VB = KT * ES;            // bytes of a V row in a tile
+  constexpr int TILE = KT * RB;          // bytes of K, and of V, in a tile
+  constexpr int NC = TILE / 1024;        // copies of K, and of V
+  constexpr int KC = D / 32;
+  constexpr int MT = D / 16;
+  constexpr int U = SP_UNIT;
+  constexpr int MROW = D + 4;            // floats a row where sums are added
+  static_assert(W * KT == U && W * 2 * TILE <= tiles_bytes(D) &&
+                W * 16 * MROW * 4 <= tiles_bytes(D) && SP_ROWS * 4 <= tiles_bytes(D), "");
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wid = uniform(tid >> 6);
+  const int l15 = lane & 15;
+  const int l4 = lane >> 4;
+  const int G = a.Hq / a.Hk, BS = 1 << a.shift;
+
+  float(*ms)[16] = (float(*)[16])(S + tiles_bytes(D));
+  float(*ls)[16] = ms + W;
+
+  // ---- this workgroup's run of units ------------------------------------------------
+  int* const units = (int*)S;  // of every row, before the tiles lie there
+  for (int b = tid; b < a.B; b += 256) {
+    const int L = a.lens[b];
+    units[b] = suffix_units(max(prefix_of(a, b), window_start(a, L)), L);
+  }
+  __syncthreads();
+  int seq = 0, at = 0, todo = 0, per = 1;
+  {
+    int total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64)
+      total += b0 + lane < a.B ? units[b0 + lane] : 0;
+    total = __shfl(scan64(total), 63, WAVE_SIZE);
+    per = max((total + a.s_runs - 1) / a.s_runs, 1);
+    const int begin = run * per;
+    if (begin >= total) return;
+    todo = min(per, total - begin);
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const int n = b0 + lane < a.B ? units[b0 + lane] : 0;
+      const int s = scan64(n);
+      const unsigned long long hit = __ballot(before + s > begin);
+      if (hit) {
+        const int src = __ffsll(hit) - 1;
+        seq = b0 + src;
+        at = begin - before - __shfl(s, src, WAVE_SIZE) + __shfl(n, src, WAVE_SIZE);
+        break;
+      }
+      before += __shfl(s, 63, WAVE_SIZE);
+    }
+  }
+  __syncthreads();  // the list is read
+  seq = uniform(seq);
+  at = uniform(at);
+  todo = uniform(todo);
+  per = uniform(per);
+  int done = 0;  // units of the run so far
+
+  uint8_t* Kt = S + wid * (2 * TILE);
+  uint8_t* Vt = Kt + TILE;
+  // ---- what a lane copies: byte offsets within a page ------------------------------
+  const uint32_t k_row = lane / CPR;
+  const uint32_t k_ch = (lane % CPR) ^ swz_k<CPR>(k_row);
+  const uint32_t v_row = lane / (VB / 16);
+  const uint32_t v_tok = ((lane % (VB / 16)) ^ swz_v<FP8>(v_row)) * (16 / ES);
+  const bool v_second = v_tok >= (uint32_t)BS;  // of two pages of 16
+  const uint32_t v_off = (v_row * BS + (v_tok & (BS - 1))) * ES;
+  const int64_t page_bytes = (int64_t)a.Hk * BS * RB;
+  const int64_t head_off = (int64_t)hk * BS * RB;
+  // ---- what a lane reads ------------------------------------------------------------
+  const int rr = 8 * (l15 >> 2) + (l15 & 3);
+  const uint32_t k_at = lds_at(Kt) + rr * RB + (l4 ^ swz_k<CPR>(rr)) * 16;
+  const uint32_t v_at =
+      FP8 ? lds_at(Vt) + l15 * VB + ((l4 >> 1) ^ swz_v<FP8>(l15)) * 16 + (l4 & 1) * 8
+          : lds_at(Vt) + l15 * VB + (l4 ^ swz_v<FP8>(l15)) * 16;
+  const float c = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1e-20f);
+
+  while (todo > 0) {
+    const int L = a.lens[seq];
+    const int P = prefix_of(a, seq);
+    const int lo = max(P, window_start(a, L));
+    const int units = suffix_units(lo, L);
+    if (at >= units) {  // a row without tokens of its own
+      ++seq;
+      at = 0;
+      continue;
+    }
+    const int t0 = at, t1 = min(units, at + todo);
+    if (t0 == 0 && hk == 0 && tid == 0)
+      a.s_info[seq] = make_int2(run, run + (done + units - 1) / per);
+    const int unit0 = lo / U;
+    const auto* table = (const __attribute__((address_space(4))) int*)(
+        a.tables + (size_t)seq * a.max_blocks);
+
+    bf16x8v qf[KC];
+    {
+      const uint16_t* row = a.q + seq * a.q_stride + (hk * G + min(l15, G - 1)) * D;
+#pragma unroll
+      for (int s = 0; s < KC; ++s)
+        qf[s] = *(const bf16x8v*)(row + (FP8 ? ((s >> 1) * 4 + l4) * 16 + (s & 1) * 8
+                                             : s * 32 + l4 * 8));
+    }
+    f32x4v o[MT] = {};
+    float m = kLowest, l = 0.f;
+
+    // this wave's tiles: from first on, a unit apart
+    int first = (unit0 + t0) * U + wid * KT;
+    if (first + KT <= lo) first += U;
+    const int end = min(L, (unit0 + t1) * U);
+    // past the end the copies are of the last tile again: the count of copies in
+    // flight stays the same
+    const int last = (L - 1) & ~(KT - 1);
+    auto pages = [&](int tok, int(&p)[2]) INL {  // of the tile's two halves
+      const int x = min(tok, last);
+      p[0] = page_at(a, table[x >> a.shift]);
+      p[1] = page_at(a, table[min(a.shift == 4 ? x + 16 : x, L - 1) >> a.shift]);
+    };
+    auto issue_k = [&](int tok, const int(&p)[2]) INL {
+      const int64_t in = head_off + (int64_t)(min(tok, last) & (BS - 1)) * RB;
+      const uint8_t* b0 = a.k + p[0] * page_bytes + in;
+      const uint8_t* b1 = a.k + p[1] * page_bytes + in;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        constexpr int RC = 64 / CPR;  // rows a copy
+        const uint32_t off = k_row * RB + (k_ch ^ swz_k<CPR>(i * RC)) * 16;
+        // the second 16 rows: of the second page, if pages have 16
+        const uint8_t* b = i < NC / 2 ? b0 + i * 1024
+                           : a.shift == 4 ? b1 + (i - NC / 2) * 1024
+                                          : b0 + i * 1024;
+        copy16_to_lds(b + off, Kt + i * 1024);
+      }
+    };
+    auto issue_v = [&](int tok, const int(&p)[2]) INL {
+      const int64_t in = head_off + (int64_t)(min(tok, last) & (BS - 1)) * ES;
+      const int64_t page = v_second ? p[1] : p[0];
+      const uint8_t* b = a.v + in + page * page_bytes + v_off;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        copy16_to_lds(b + i * (1024 / VB) * BS * ES, Vt + i * 1024);
+    };
+
+    if (first < end) {
+      int nx[2];
+      pages(first, nx);
+      issue_k(first, nx);
+      issue_v(first, nx);
+      pages(first + U, nx);
+      if (a.scale < 0.f) {  // the sign goes with q, as c takes maxima
+#pragma unroll
+        for (int s = 0; s < KC; ++s)
+          qf[s] = __builtin_bit_cast(
+              bf16x8v, __builtin_bit_cast(u32x4v, qf[s]) ^ 0x80008000u);
+      }
+      for (int tok = first; tok < end; tok += U) {
+        wait_copies<NC>();
+        u32x4v kr[KC * ES];  // [chunk group][t]
+        if constexpr (CPR == 16)
+          read8<4 * RB>(kr, k_at, k_at ^ 64, k_at ^ 128, k_at ^ 192);
+        else if constexpr (CPR == 8)
+          read4<4 * RB>(kr, k_at, k_at ^ 64);
+        else
+          read2<4 * RB>(kr, k_at);
+        issue_k(tok + U, nx);
+
+        // token of s[t][r]: tok + 8 l4 + 4 t + r
+        f32x4v s[2] = {};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int k = 0; k < KC; ++k) {
+            bf16x8v x;
+            if constexpr (FP8) {
+              const u32x4v r = kr[(k >> 1) * 2 + t];
+              x = k & 1 ? widen(r[2], r[3]) : widen(r[0], r[1]);
+            } else {
+              x = __builtin_bit_cast(bf16x8v, kr[k * 2 + t]);
+            }
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qf[k], s[t], 0, 0, 0);
+          }
+        if (a.softcap > 0.f) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            s[e >> 2][e & 3] = a.softcap *
+                               tanhf(s[e >> 2][e & 3] * fabsf(a.scale) / a.softcap) *
+                               kLog2e;
+        }
+        const bool cut = tok + KT > L || tok < lo;
+        if (cut) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int k = tok + 8 * l4 + e;
+            s[e >> 2][e & 3] = k >= lo && k < L ? s[e >> 2][e & 3] : kHidden;
+          }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
+        mx = over_head(mx, [](float x, float y) { return fmaxf(x, y); }) * c;
+        if (__any(mx > m)) {
+          const float m2 = fmaxf(m, mx);
+          const float f = __builtin_amdgcn_exp2f(m - m2);
+          m = m2;
+          l *= f;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) o[t] *= f;
+        }
+        u32x4v pk;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], c, -m));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][(e & 3) + 1], c, -m));
+          l += p0 + p1;
+          pk[e >> 1] = pack_bf16(p0, p1);
+        }
+
+        wait_copies<NC>();
+        using VR = std::conditional_t<FP8, u32x2v, u32x4v>;
+        VR vr[MT];
+        read_rows(vr, v_at);
+        issue_v(tok + U, nx);
+        pages(tok + 2 * U, nx);
+        // slots past the end, and before the row's own tokens, may hold anything:
+        // weight 0 times it
+        u32x4v keep = {~0u, ~0u, ~0u, ~0u};
+        if (cut) {
+          const int from = lo - tok - 8 * l4, to = L - tok - 8 * l4;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            keep[i] = (2 * i >= from && 2 * i < to ? 0xffffu : 0u) |
+                      (2 * i + 1 >= from && 2 * i + 1 < to ? 0xffff0000u : 0u);
+        }
+        const bf16x8v pb = __builtin_bit_cast(bf16x8v, pk);
+#pragma unroll
+        for (int d = 0; d < MT; ++d) {
+          u32x4v x;
+          if constexpr (FP8)
+            x = __builtin_bit_cast(u32x4v, widen(vr[d][0], vr[d][1]));
+          else
+            x = vr[d];
+          if (cut) x &= keep;
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8v, x), pb, o[d], 0, 0, 0);
+        }
+      }
+      wait_copies<0>();
+    }
+
+    // ---- the waves' sums -------------------------------------------------------------
+    l = over_head(l, [](float x, float y) { return x + y; });
+    if (l4 == 0) {
+      ms[wid][l15] = m;
+      ls[wid][l15] = l;
+    }
+    __syncthreads();
+    float M = kLowest;
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, ms[w][l15]);
+    const float f = __builtin_amdgcn_exp2f(m - M);
+    float* sums = reinterpret_cast<float*>(S);
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+      *reinterpret_cast<f32x4v*>(sums + (wid * 16 + l15) * MROW + t * 16 + l4 * 4) =
+          o[t] * f;
+    __syncthreads();
+    const bool whole = P == 0 && t0 == 0 && t1 == units;
+    for (int e = tid; e < G * (D / 4); e += W * 64) {
+      const int g = e / (D / 4), d = e % (D / 4) * 4;
+      float Mg = kLowest, lg = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) Mg = fmaxf(Mg, ms[w][g]);
+#pragma unroll
+      for (int w = 0; w < W; ++w) lg += ls[w][g] * __builtin_amdgcn_exp2f(ms[w][g] - Mg);
+      f32x4v s = {};
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        s += *reinterpret_cast<const f32x4v*>(sums + (w * 16 + g) * MROW + d);
+      const int h = hk * G + g;
+      if (whole) {
+        if (a.sinks != nullptr) lg += __builtin_amdgcn_exp2f(a.sinks[h] * kLog2e - Mg);
+        s *= a.v_scale / lg;
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)seq * a.Hq + h) * D + d) =
+            make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
+      } else {
+        const int64_t part = (int64_t)(run + seq) * a.Hq + h;
+        *reinterpret_cast<f32x4v*>(a.s_acc + part * D + d) = s;
+        if (d == 0) *reinterpret_cast<f32x2v*>(a.s_ml + part * 2) = f32x2v{Mg, lg};
+      }
+    }
+    __syncthreads();
+    todo -= t1 - t0;
+    done += t1 - t0;
+    ++seq;
+    at = 0;
+  }
+}
+
+}  // namespace
+
+template <int D, bool FP8>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(
+    const SharedPrefix a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t S[lds_bytes(D)];
+  const int hk = blockIdx.x % a.Hk, run = blockIdx.x / a.Hk;
+  if (run < a.p_runs) prefix_role<D, FP8>(a, S, hk, run);
+  else suffix_role<D, FP8>(a, S, hk, run - a.p_runs);
+}
+
+// Joins the parts of every row and query head: a wave each. Lanes take a part each for
+// the weights, then groups of D / 4 lanes the parts in turn, in a fixed order.
+template <int D>
+__global__ __launch_bounds__(256) void shared_prefix_join_kernel(const SharedPrefix a) {
+  const int lane = threadIdx.x & 63;
+  const int h = blockIdx.x * 4 + (threadIdx.x >> 6), b = blockIdx.y;
+  if (h >= a.Hq) return;
+  const int G = a.Hq / a.Hk, hk = h / G;
+  const int L = a.lens[b], P = prefix_of(a, b);
+  constexpr int Q = D / 4, GROUPS = 64 / Q;
+  const int d = lane % Q * 4, grp = lane / Q;
+  uint16_t* out = a.out + ((int64_t)b * a.Hq + h) * D + d;
+  const int su = suffix_units(max(P, window_start(a, L)), L);
+  if (P == 0 && su == 0) {  // no tokens: zeros
+    if (grp == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
+    return;
+  }
+  int2 sr = make_int2(0, -1);
+  if (su > 0) sr = a.s_info[b];
+  if (P == 0 && sr.x == sr.y) return;  // finished by its run
+  int4 pi = make_int4(0, 0, 0, 0);
+  if (P > 0) pi = a.p_info[(int64_t)b * a.Hq + h];
+  const int np = pi.y, parts = np + sr.y - sr.x + 1;
+  // where part i lies
+  auto at = [&](int i, const float** ml, const float** acc) INL {
+    const int64_t x = i < np ? ((int64_t)(pi.x + i) * a.Hk + hk) * SP_ITEMS + pi.z
+                             : (int64_t)(sr.x + i - np + b) * a.Hq + h;
+    *ml = (i < np ? a.p_ml : a.s_ml) + x * 2;
+    *acc = (i < np ? a.p_acc : a.s_acc) + x * D;
+  };
+  float M = kLowest, l = 0.f;
+  f32x4v s = {};
+  for (int i0 = 0; i0 < parts; i0 += 64) {
+    const float *ml, *acc;
+    f32x2v v = {kLowest, 0.f};
+    if (i0 + lane < parts) {
+      at(i0 + lane, &ml, &acc);
+      v = *reinterpret_cast<const f32x2v*>(ml);
+    }
+    const float M2 = fmaxf(M, wave_reduce_max(v[0]));
+    const float f = __builtin_amdgcn_exp2f(M - M2);
+    const float w = __builtin_amdgcn_exp2f(v[0] - M2);
+    M = M2;
+    l = l * f + wave_reduce_sum(v[1] * w);
+    s *= f;
+    const int n = min(64, parts - i0);
+#pragma unroll 4
+    for (int i = 0; i < n; i += GROUPS) {
+      const int mine = min(i + grp, n - 1);
+      const float x = __shfl(w, mine, WAVE_SIZE);
+      at(i0 + mine, &ml, &acc);
+      const f32x4v y = *reinterpret_cast<const f32x4v*>(acc + d);
+      s += y * (i + grp < n ? x : 0.f);
+    }
+  }
+#pragma unroll
+  for (int o = Q; o < 64; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += __shfl_xor(s[e], o, WAVE_SIZE);
+  if (a.sinks != nullptr) l += __builtin_amdgcn_exp2f(a.sinks[h] * kLog2e - M);
+  s *= a.v_scale / l;
+  if (grp == 0)
+    *reinterpret_cast<uint2*>(out) =
+        make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
+}
+
+// Workgroups of a key/value head for prefixes and for suffixes, and the item tiles that
+// B rows of N groups make at most.
+extern "C" void shared_prefix_plan(int B, int N, int Hq, int Hk, int D, int* p_runs,
+                                   int* s_runs, int* tiles) {
+  const int slots = std::max(1, (D == 128 ? 256 : 512) / Hk);
+  *p_runs = N > 0 ? slots : 0;
+  *s_runs = slots;
+  *tiles = N > 0 ? (int)((int64_t)B * (Hq / Hk) / SP_ITEMS) + std::min(N, B) : 0;
 }
 
 extern "C" void launch_shared_prefix(const SharedPrefix* a, bool fp8, hipStream_t stream) {
-  const dim3 grid(a->Hq, a->B);
-  auto run = [&](auto kernel) { kernel<<<grid, 64, 0, stream>>>(*a); };
-  fp8 ? run(shared_prefix_kernel<true>) : run(shared_prefix_kernel<false>);
+  const dim3 grid((a->p_runs + a->s_runs) * a->Hk);
+  auto run = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(*a); };
+  if (a->D == 128) fp8 ? run(shared_prefix_kernel<128, true>)
+                       : run(shared_prefix_kernel<128, false>);
+  else fp8 ? run(shared_prefix_kernel<64, true>) : run(shared_prefix_kernel<64, false>);
+  const dim3 heads((a->Hq + 3) / 4, a->B);
+  auto join = [&](auto kernel) { kernel<<<heads, 256, 0, stream>>>(*a); };
+  a->D == 128 ? join(shared_prefix_join_kernel<128>) : join(shared_prefix_join_kernel<64>);
 }

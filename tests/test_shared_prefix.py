@@ -97,6 +97,10 @@ def test_too_many_rows():
                 q=torch.zeros(n, 4, 64).bfloat16(), seq_lens=torch.zeros(n, dtype=i),
                 block_tables=torch.zeros(n, 1, dtype=i),
                 prefix_group=torch.zeros(n, dtype=i))))
+    with pytest.raises(RuntimeError, match="256 groups"):
+        ops._require_ext("test").shared_prefix_attention_decode(
+            *arguments(prefix_inputs(4, 2, 64, 16, [(0, 40)], [20]), dict(
+                prefix_lens=torch.zeros(257, dtype=i))))
 
 
 @EXT

@@ -108,7 +108,7 @@ def test_no_groups(rows):
 
 def test_most_rows():
     rows = shared(4096, 20, 12)
-    check(prefix_inputs(2, 1, 64, 16, rows, [20] + [7] * 4095))
+    check(prefix_inputs(2, 1, 64, 16, rows, [20] + [7] * 255))
 
 
 def test_empty_batch_of_rows():
