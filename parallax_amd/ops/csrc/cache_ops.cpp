@@ -41,7 +41,8 @@ struct SharedPrefix {
   int64_t q_stride;
   float scale, v_scale, softcap;
   int window;
-  int p_runs, s_runs;
+  int runs;
+  float ratio;
   float *p_acc, *p_ml;
   int4* p_info;
   float *s_acc, *s_ml;
@@ -50,7 +51,7 @@ struct SharedPrefix {
 
 extern "C" {
 void launch_head_norm_store(const HeadNormStore*, bool, bool, hipStream_t);
-void shared_prefix_plan(int, int, int, int, int, int*, int*, int*);
+void shared_prefix_plan(int, int, int, int, int, int*, int*);
 void launch_shared_prefix(const SharedPrefix*, bool, hipStream_t);
 }
 
@@ -200,10 +201,10 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   check_list(prefix_lens, at::kInt, N, "prefix_lens");
   TORCH_CHECK(B <= 4096 && N <= 256, "at most 4096 rows and 256 groups");
   const int64_t max_blocks = block_tables.size(1);
-  // key tiles of all item tiles, and units of all rows, are counted in 32 bits
+  // key tiles of all item tiles, and suffix tiles of all rows, are counted in 32 bits
   TORCH_CHECK(max_blocks * BS < INT_MAX / 4 &&
-                  (B * Hq / Hk / 128 + N) * (max_blocks * BS / 64 + 1) < INT_MAX &&
-                  B * (max_blocks * BS / 128 + 1) < INT_MAX &&
+                  (B * Hq / Hk / 128 + N) * (max_blocks * BS / 64 + 1) < INT_MAX / 2 &&
+                  B * (max_blocks * BS / 32 + 1) < INT_MAX / 2 &&
                   Hk * BS * D <= INT_MAX && Hq <= 65535,
               "too many tokens or heads");
   TORCH_CHECK(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0,
@@ -243,11 +244,11 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   a.softcap = (float)softcap;
   a.window = sliding_window > 0 ? (int)std::min<int64_t>(sliding_window, INT_MAX) : 0;
   int tiles;
-  shared_prefix_plan(a.B, a.N, a.Hq, a.Hk, a.D, &a.p_runs, &a.s_runs, &tiles);
+  shared_prefix_plan(a.B, a.N, a.Hq, a.Hk, a.D, &a.runs, &tiles);
   // fp32 words: of a part its sums, then maxima and sums of weights; then where a row's
   // parts lie
-  const int64_t p_items = N > 0 ? (int64_t)(a.p_runs + tiles) * Hk * 128 : 0;
-  const int64_t s_items = (a.s_runs + B) * Hq;
+  const int64_t p_items = N > 0 ? (int64_t)(a.runs + tiles) * Hk * 128 : 0;
+  const int64_t s_items = (4 * a.runs + B) * Hq;
   const int64_t words = (p_items + s_items) * (D + 2) + B * Hq * 4 + B * 2;
   auto work = torch::empty({words}, q.options().dtype(at::kFloat));
   float* at = work.data_ptr<float>();

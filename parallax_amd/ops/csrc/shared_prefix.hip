@@ -19,14 +19,15 @@
 //
 // Suffixes. The tokens behind the prefix (of a row without a group: all) are decode
 // attention as in paged_decode.hip: a wave copies tiles of 32 tokens into LDS of its
-// own, a key/value head's query heads are 16 columns; units of 128 tokens of all rows
-// form one list, dealt in equal runs.
+// own, a key/value head's query heads are 16 columns. The tiles of all rows form one
+// list, dealt in equal runs to the waves, which never wait for each other.
 //
 // Lengths, groups and prefixes are read on the device, by every workgroup itself; the
 // grid depends on sizes alone.
 
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 
 #include "common.h"
 #include "decode_common.h"
@@ -34,7 +35,7 @@
 
 #define SP_KT 64       // keys of a prefix tile
 #define SP_ITEMS 128   // items of one
-#define SP_UNIT 128    // tokens of a suffix unit: 32 a wave
+#define SP_UNIT 32     // tokens of a suffix tile
 #define SP_GROUPS 256  // at most
 #define SP_ROWS 4096   // at most
 
@@ -50,14 +51,14 @@ struct SharedPrefix {
   int64_t q_stride;
   float scale, v_scale, softcap;  // scale: with that of an fp8 cache's keys
   int window;
-  // workgroups of a key/value head: for prefixes, for suffixes
-  int p_runs, s_runs;
+  int runs;      // workgroups of a key/value head
+  float ratio;
   float* p_acc;  // [p_parts, Hk, SP_ITEMS, D]: part run + item tile
   float* p_ml;   // [p_parts, Hk, SP_ITEMS, 2] maxima in units of log2, sums
   int4* p_info;  // [B, Hq]: first part, parts, place in them; rows of a group only
-  float* s_acc;  // [s_runs + B, Hq, D]: part run + row
-  float* s_ml;   // [s_runs + B, Hq, 2]
-  int2* s_info;  // [B]: first and last run; rows with tokens behind a prefix only
+  float* s_acc;  // [s_parts, Hq, D]: part wave + row
+  float* s_ml;   // [s_parts, Hq, 2]
+  int2* s_info;  // [B]: first and last wave; rows with tokens behind a prefix only
 };
 
 namespace {
@@ -72,7 +73,7 @@ DEVINL int window_start(const SharedPrefix& a, int L) {
   return a.window > 0 ? max(0, L - a.window) : 0;
 }
 
-// units of a row's tokens [lo, L)
+// suffix tiles of a row's tokens [lo, L)
 DEVINL int suffix_units(int lo, int L) {
   return L > lo ? (L + SP_UNIT - 1) / SP_UNIT - lo / SP_UNIT : 0;
 }
@@ -92,13 +93,32 @@ DEVINL float over_halves(float v, F f) {
 
 constexpr int tiles_bytes(int D) { return 4 * SP_KT * D * 2; }
 constexpr int lds_bytes(int D) {
-  return tiles_bytes(D) + (2 * SP_GROUPS + SP_ITEMS + 4) * 4 + SP_ROWS * 2;
+  return tiles_bytes(D) + (3 * SP_GROUPS + SP_ITEMS + 4) * 4 + SP_ROWS * 2;
 }
+
+// What a workgroup finds of the batch, in LDS behind its tiles.
+struct Lists {
+  int* prefix;      // the groups' lengths
+  int* count;       // rows of a group
+  int* low;         // where the first window of a group's rows begins
+  int* rows;        // of an item tile; [SP_ITEMS]: its group's first row
+  int16_t* member;  // a row's group, -1: none
+  int* units;       // a row's suffix tiles; here the tiles come to lie
+
+  // item tiles of a group, and its key tiles [*begin, result), one at least
+  DEVINL int tiles(int g, int G) const { return (count[g] * G + SP_ITEMS - 1) / SP_ITEMS; }
+  DEVINL int keys(int g, int* begin) const {
+    const int end = (prefix[g] + SP_KT - 1) / SP_KT;
+    *begin = min(low[g] / SP_KT, end - 1);
+    return end;
+  }
+};
 
 // ---- prefixes ----------------------------------------------------------------------
 
 template <int D, bool FP8>
-DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const int run) {
+DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const int hk,
+                        const int run, const int total, const int runs) {
   constexpr int KCH = D / 8;            // 16-byte chunks of a K row
   constexpr int KPER = SP_KT * KCH / 256;  // chunks that a thread copies
   constexpr int VPER = D * 8 / 256;
@@ -115,74 +135,35 @@ DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
   uint16_t* const V0 = K0 + SP_KT * D;
   uint16_t* const K1 = V0 + SP_KT * D;
   uint16_t* const V1 = K1 + SP_KT * D;
-  int* const count = (int*)(S + tiles_bytes(D));  // rows of a group
-  int* const low = count + SP_GROUPS;             // where the first window begins
-  int* const rows = low + SP_GROUPS;              // of an item tile; 130: the group's first
-  int16_t* const member = (int16_t*)(rows + SP_ITEMS + 4);  // a row's group
-
-  for (int g = tid; g < a.N; g += 256) {
-    count[g] = 0;
-    low[g] = INT_MAX;
-  }
-  __syncthreads();
-  for (int b = tid; b < a.B; b += 256) {
-    const int p = prefix_of(a, b);
-    const int g = p > 0 ? a.group[b] : -1;
-    member[b] = (int16_t)g;
-    if (g >= 0) {
-      atomicAdd(count + g, 1);
-      atomicMin(low + g, window_start(a, a.lens[b]));
-    }
-  }
-  __syncthreads();
 
   // ---- this workgroup's run of key tiles ------------------------------------------
-  auto tiles_of = [&](int g) { return (count[g] * G + SP_ITEMS - 1) / SP_ITEMS; };
-  auto keys_of = [&](int g, int* begin) {  // at least one tile
-    const int end = (a.prefix[g] + SP_KT - 1) / SP_KT;
-    *begin = min(low[g] / SP_KT, end - 1);
-    return end;
-  };
-  int g = 0, at = 0, tile0 = 0, todo = 0, per = 1, begin = 0;
-  {
-    int total = 0;
-    for (int g0 = 0; g0 < a.N; g0 += 64) {
-      const int x = g0 + lane;
-      int kb, n = 0;
-      if (x < a.N && count[x] > 0) n = tiles_of(x) * (keys_of(x, &kb) - kb);
-      total += __shfl(scan64(n), 63, WAVE_SIZE);
+  const int per = max((total + runs - 1) / runs, 1);
+  const int begin = run * per;
+  if (begin >= total) return;
+  int todo = min(per, total - begin);
+  int g = 0, at = 0, tile0 = 0, before = 0;
+  for (int g0 = 0; g0 < a.N; g0 += 64) {
+    const int x = g0 + lane;
+    int kb, n = 0, t = 0;
+    if (x < a.N && w.count[x] > 0) {
+      t = w.tiles(x, G);
+      n = t * (w.keys(x, &kb) - kb);
     }
-    per = max((total + a.p_runs - 1) / a.p_runs, 1);
-    begin = run * per;
-    if (begin >= total) return;
-    todo = min(per, total - begin);
-    int before = 0;
-    for (int g0 = 0; g0 < a.N; g0 += 64) {
-      const int x = g0 + lane;
-      int kb, n = 0, t = 0;
-      if (x < a.N && count[x] > 0) {
-        t = tiles_of(x);
-        n = t * (keys_of(x, &kb) - kb);
-      }
-      const int ns = scan64(n), ts = scan64(t);
-      const unsigned long long hit = __ballot(before + ns > begin);
-      if (hit) {
-        const int src = __ffsll(hit) - 1;
-        g = g0 + src;
-        at = begin - before - __shfl(ns, src, WAVE_SIZE) + __shfl(n, src, WAVE_SIZE);
-        tile0 += __shfl(ts, src, WAVE_SIZE) - __shfl(t, src, WAVE_SIZE);
-        break;
-      }
-      before += __shfl(ns, 63, WAVE_SIZE);
-      tile0 += __shfl(ts, 63, WAVE_SIZE);
+    const int ns = scan64(n), ts = scan64(t);
+    const unsigned long long hit = __ballot(before + ns > begin);
+    if (hit) {
+      const int src = __ffsll(hit) - 1;
+      g = g0 + src;
+      at = begin - before - __shfl(ns, src, WAVE_SIZE) + __shfl(n, src, WAVE_SIZE);
+      tile0 += __shfl(ts, src, WAVE_SIZE) - __shfl(t, src, WAVE_SIZE);
+      break;
     }
+    before += __shfl(ns, 63, WAVE_SIZE);
+    tile0 += __shfl(ts, 63, WAVE_SIZE);
   }
   g = uniform(g);
   at = uniform(at);
   tile0 = uniform(tile0);
-  todo = uniform(todo);
-  per = uniform(per);
-  begin = uniform(begin);
 
   // ---- what a lane copies and reads -------------------------------------------------
   // 16 chunks (256 bytes) make a turn over the banks: a K row of 128 values, or two of
@@ -214,10 +195,10 @@ DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
 
   int done = 0;
   while (todo > 0) {
-    const int n_items = count[g] * G;
-    const int P = a.prefix[g];
+    const int n_items = w.count[g] * G;
+    const int P = uniform(w.prefix[g]);
     int kb;
-    const int kend = uniform(keys_of(g, &kb));
+    const int kend = uniform(w.keys(g, &kb));
     kb = uniform(kb);
     const int keys = kend - kb;
     const int tile = at / keys;
@@ -230,11 +211,11 @@ DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
     if (wid == 0) {
       int rank = 0;
       for (int b0 = 0; b0 < a.B && rank <= r1; b0 += 64) {
-        const bool is = b0 + lane < a.B && member[b0 + lane] == g;
+        const bool is = b0 + lane < a.B && w.member[b0 + lane] == g;
         const unsigned long long all = __ballot(is);
         const int mine = rank + __popcll(all & ((1ull << lane) - 1));
-        if (is && mine >= r0 && mine <= r1) rows[mine - r0] = b0 + lane;
-        if (is && mine == 0) rows[SP_ITEMS + 2] = b0 + lane;
+        if (is && mine >= r0 && mine <= r1) w.rows[mine - r0] = b0 + lane;
+        if (is && mine == 0) w.rows[SP_ITEMS] = b0 + lane;
         rank += __popcll(all);
       }
     }
@@ -242,19 +223,19 @@ DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
     const int item = tile * SP_ITEMS + wid * 32 + l31;
     const bool on = item < n_items;
     const int r = min(item, n_items - 1) / G;
-    const int row = rows[r - r0];
+    const int row = w.rows[r - r0];
     const int h = hk * G + min(item, n_items - 1) - r * G;
     const int lo = window_start(a, a.lens[row]);
     // constant memory: read by the scalar unit
     const auto* table = (const __attribute__((address_space(4))) int*)(
-        a.tables + (size_t)uniform(rows[SP_ITEMS + 2]) * a.max_blocks);
+        a.tables + (size_t)uniform(w.rows[SP_ITEMS]) * a.max_blocks);
     const bool wave_on = tile * SP_ITEMS + wid * 32 < n_items;
     int lo_most = lo;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
       lo_most = max(lo_most, __shfl_xor(lo_most, o, WAVE_SIZE));
     lo_most = uniform(lo_most);
-    const int lo_least = low[g];
+    const int lo_least = w.low[g];
 
     if (k0 == kb && half == 0 && on)
       a.p_info[(int64_t)row * a.Hq + h] =
@@ -272,12 +253,14 @@ DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
       }
     }
 
+    // Pages of the rows and chunks that this thread copies next: K's of tile kt, V's of
+    // tile vt. Tokens past the end are hidden later; their place is in the last page.
     int kpage = 0, vpage[2] = {0, 0};
-    auto pages = [&](int kt) INL {  // of the rows and chunks that this thread copies
+    const int* vtable = (const int*)table;
+    auto pages = [&](int kt, int vt) INL {
       kpage = page_at(a, table[min(kt * SP_KT + wid * 16, P - 1) >> a.shift]);
-      const int* t = (const int*)table;
-      vpage[0] = page_at(a, t[min(kt * SP_KT + v_src(0) * 8, P - 1) >> a.shift]);
-      vpage[1] = page_at(a, t[min(kt * SP_KT + v_src(1) * 8, P - 1) >> a.shift]);
+      vpage[0] = page_at(a, vtable[min(vt * SP_KT + v_src(0) * 8, P - 1) >> a.shift]);
+      vpage[1] = page_at(a, vtable[min(vt * SP_KT + v_src(1) * 8, P - 1) >> a.shift]);
     };
     auto k_elem = [&](int i) INL {
       return (uint64_t)(uint32_t)kpage * page_elems + (uint32_t)koff[i];
@@ -285,103 +268,104 @@ DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
     auto v_elem = [&](int i) INL {
       return (uint64_t)(uint32_t)vpage[i & 1] * page_elems + (uint32_t)voff[i];
     };
-    uint64_t kraw[FP8 ? KPER : 1], vraw[FP8 ? VPER : 1];
-    auto issue = [&](uint16_t* Kl, uint16_t* Vl) INL {
-      if constexpr (FP8) {
-#pragma unroll
-        for (int i = 0; i < KPER; ++i)
-          kraw[i] = *reinterpret_cast<const uint64_t*>(a.k + k_elem(i));
-#pragma unroll
-        for (int i = 0; i < VPER; ++i)
-          vraw[i] = *reinterpret_cast<const uint64_t*>(a.v + v_elem(i));
-      } else {
-#pragma unroll
-        for (int i = 0; i < KPER; ++i)
-          copy16_to_lds((const uint16_t*)a.k + k_elem(i), Kl + (wid * KPER + i) * 512);
-#pragma unroll
-        for (int i = 0; i < VPER; ++i)
-          copy16_to_lds((const uint16_t*)a.v + v_elem(i), Vl + (wid * VPER + i) * 512);
-      }
+    auto copy_k = [&](uint16_t* Kl, int i) INL {
+      copy16_to_lds((const uint16_t*)a.k + k_elem(i), Kl + (wid * KPER + i) * 512);
     };
-    auto settle = [&](uint16_t* Kl, uint16_t* Vl) INL {  // fp8: what was asked for
-      if constexpr (FP8) {
+    auto copy_v = [&](uint16_t* Vl, int i) INL {
+      copy16_to_lds((const uint16_t*)a.v + v_elem(i), Vl + (wid * VPER + i) * 512);
+    };
+    uint64_t kraw[FP8 ? KPER : 1], vraw[FP8 ? VPER : 1];  // fp8 passes registers
+    auto fetch_k = [&]() INL {
 #pragma unroll
-        for (int i = 0; i < KPER; ++i)
-          *reinterpret_cast<bf16x8v*>(Kl + ((wid * KPER + i) * 64 + lane) * 8) =
-              widen((uint32_t)kraw[i], (uint32_t)(kraw[i] >> 32));
+      for (int i = 0; i < KPER; ++i)
+        kraw[i] = *reinterpret_cast<const uint64_t*>(a.k + k_elem(i));
+    };
+    auto fetch_v = [&]() INL {
 #pragma unroll
-        for (int i = 0; i < VPER; ++i)
-          *reinterpret_cast<bf16x8v*>(Vl + ((wid * VPER + i) * 64 + lane) * 8) =
-              widen((uint32_t)vraw[i], (uint32_t)(vraw[i] >> 32));
-      }
+      for (int i = 0; i < VPER; ++i)
+        vraw[i] = *reinterpret_cast<const uint64_t*>(a.v + v_elem(i));
+    };
+    auto settle_k = [&](uint16_t* Kl) INL {
+#pragma unroll
+      for (int i = 0; i < KPER; ++i)
+        *reinterpret_cast<bf16x8v*>(Kl + ((wid * KPER + i) * 64 + lane) * 8) =
+            widen((uint32_t)kraw[i], (uint32_t)(kraw[i] >> 32));
+    };
+    auto settle_v = [&](uint16_t* Vl) INL {
+#pragma unroll
+      for (int i = 0; i < VPER; ++i)
+        *reinterpret_cast<bf16x8v*>(Vl + ((wid * VPER + i) * 64 + lane) * 8) =
+            widen((uint32_t)vraw[i], (uint32_t)(vraw[i] >> 32));
     };
 
-    f32x16v o[DT] = {};
-    float m = kLowest, l = 0.f;
-    auto turn = [&](int kt, const uint16_t* Kl, const uint16_t* Vl, uint16_t* Kn,
-                    uint16_t* Vn) INL {
+    f32x16v o[DT] = {}, s0[2] = {}, s1[2];
+    float m = kLowest, l = 0.f, lsum = 0.f;
+    float mx = kLowest;  // of the scores whose weights come next
+    // weights of two tokens, part j of a B operand of 16
+    auto weigh = [&](const f32x16v(&s)[2], int ks, int j) INL {
+      const int e = (ks & 1) * 8 + 2 * j;
+      const float x = __builtin_amdgcn_exp2f(fmaf(s[ks >> 1][e], c, -m));
+      const float y = __builtin_amdgcn_exp2f(fmaf(s[ks >> 1][e + 1], c, -m));
+      lsum += x;
+      lsum += y;
+      return pack_bf16(x, y);
+    };
+    auto larger = [](float x, const f32x16v& s) INL {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x = fmaxf(x, s[e]);
+      return x;
+    };
+    auto top_of = [&](float x) INL {
+      return over_halves(x, [](float p, float q) { return fmaxf(p, q); }) * c;
+    };
+    // rescaled when a maximum moved: its own weight is then 1, without error
+    auto raise = [&]() INL {
+      if (__any(mx > m)) {
+        const float m2 = fmaxf(m, mx);
+        const float f = __builtin_amdgcn_exp2f(m - m2);
+        m = m2;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[t][e] *= f;
+      }
+    };
+    auto meet = [&]() INL {  // all copies and stores to LDS, of all waves
       asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0x0070);  // all copies, all stores to LDS
+      __builtin_amdgcn_s_waitcnt(0x0070);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (kt + 1 < k1) {
-        issue(Kn, Vn);
-        pages(min(kt + 2, k1 - 1));
+    };
+
+    // A turn takes the scores of tile kt and the weights and values of the tile before,
+    // which depend on nothing of this turn. Any turn: also the first and the last, a
+    // softcap, a mask.
+    auto cut_turn = [&](int kt, const uint16_t* Kl, uint16_t* Kn, const uint16_t* Vl,
+                        uint16_t* Vn) INL {
+      meet();
+      const bool more = kt < k1;
+      if (more) {  // past the last tile K's copy is the last again
+        if constexpr (FP8) {
+          fetch_k();
+          fetch_v();
+        } else {
+#pragma unroll
+          for (int i = 0; i < KPER; ++i) copy_k(Kn, i);
+#pragma unroll
+          for (int i = 0; i < VPER; ++i) copy_v(Vn, i);
+        }
+        pages(min(kt + 2, k1 - 1), min(kt + 1, k1 - 1));
       }
-      if (wave_on) {
-        const int base = kt * SP_KT;
-        f32x16v s[2] = {};
-#pragma unroll
-        for (int ks = 0; ks < KSTEPS; ++ks)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(Kl, ks, t), qf[ks],
-                                                           s[t], 0, 0, 0);
-        if (a.softcap > 0.f) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              s[t][e] = a.softcap * tanhf(s[t][e] * fabsf(a.scale) / a.softcap) * kLog2e;
-        }
+      if (wave_on && kt > k0) {
+        const int base = (kt - 1) * SP_KT;
         const bool cut = base + SP_KT > P || base < lo_least;
-        if (cut || base < lo_most) {
-          const int end = P - base - 8 * half, first = lo - base - 8 * half;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int tok = 32 * t + 16 * (e >> 3) + (e & 7);
-              s[t][e] = tok < end && tok >= first ? s[t][e] : kHidden;
-            }
-        }
-        float mx = s[0][0];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
-        mx = over_halves(mx, [](float x, float y) { return fmaxf(x, y); }) * c;
-        // rescaled when a maximum moved: its own weight is then 1, without error
-        if (__any(mx > m)) {
-          const float m2 = fmaxf(m, mx);
-          const float f = __builtin_amdgcn_exp2f(m - m2);
-          m = m2;
-          l *= f;
-#pragma unroll
-          for (int t = 0; t < DT; ++t) o[t] *= f;
-        }
+        raise();
 #pragma unroll
         for (int ks = 0; ks < SP_KT / 16; ++ks) {
           u32x4v w;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int e = (ks & 1) * 8 + 2 * j;
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[ks >> 1][e], c, -m));
-            const float y = __builtin_amdgcn_exp2f(fmaf(s[ks >> 1][e + 1], c, -m));
-            l += x;
-            l += y;
-            w[j] = pack_bf16(x, y);
-          }
+          for (int j = 0; j < 4; ++j) w[j] = weigh(s0, ks, j);
           bf16x8v v[DT];
 #pragma unroll
           for (int t = 0; t < DT; ++t) v[t] = v_frag(Vl, ks, t);
@@ -399,17 +383,122 @@ DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
             o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 v[t], __builtin_bit_cast(bf16x8v, w), o[t], 0, 0, 0);
         }
+        l += lsum;
+        lsum = 0.f;
       }
-      if (kt + 1 < k1) settle(Kn, Vn);
+      if (wave_on && more) {
+        const int base = kt * SP_KT;
+        s0[0] = s0[1] = f32x16v{};
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            s0[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(Kl, ks, t), qf[ks],
+                                                            s0[t], 0, 0, 0);
+        if (a.softcap > 0.f) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              s0[t][e] =
+                  a.softcap * tanhf(s0[t][e] * fabsf(a.scale) / a.softcap) * kLog2e;
+        }
+        if (base + SP_KT > P || base < lo_most) {
+          int end = P - base - 8 * half, first = lo - base - 8 * half;
+          asm volatile("" : "+v"(end));  // not computed where no mask is applied
+          asm volatile("" : "+v"(first));
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int tok = 32 * t + 16 * (e >> 3) + (e & 7);
+              s0[t][e] = tok < end && tok >= first ? s0[t][e] : kHidden;
+            }
+        }
+        mx = top_of(larger(larger(s0[0][0], s0[0]), s0[1]));
+      }
+      if constexpr (FP8)
+        if (more) {
+          settle_k(Kn);
+          settle_v(Vn);
+        }
     };
 
-    pages(k0);
-    issue(K0, V0);
-    settle(K0, V0);
-    pages(min(k0 + 1, k1 - 1));
-    for (int kt = k0; kt < k1; kt += 2) {
-      turn(kt, K0, V0, K1, V1);
-      if (kt + 1 < k1) turn(kt + 1, K1, V1, K0, V0);
+    // A tile seen whole behind another. The order is the one that is written here, a
+    // matrix instruction and what fits beside it at a time, operands read AHEAD
+    // instructions early; the compiler's own puts every read right before its use.
+    auto whole_turn = [&](int kt, const uint16_t* Kl, uint16_t* Kn, const uint16_t* Vl,
+                          uint16_t* Vn, f32x16v(&sn)[2], const f32x16v(&sp)[2]) INL {
+      meet();
+      raise();
+      constexpr int NS = 2 * KSTEPS, NM = NS + 4 * DT, AHEAD = 4;
+      bf16x8v fr[AHEAD];
+      u32x4v w[4];
+      auto load = [&](int n) INL {
+        fr[n % AHEAD] = n < NS ? k_frag(Kl, n % KSTEPS, n / KSTEPS)
+                               : v_frag(Vl, (n - NS) / DT, (n - NS) % DT);
+      };
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) load(n);
+      if constexpr (FP8) {
+        fetch_k();
+        fetch_v();
+        pages(min(kt + 2, k1 - 1), min(kt + 1, k1 - 1));
+      }
+#pragma unroll
+      for (int n = 0; n < NM; ++n) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (n < NS) {
+          const int t = n / KSTEPS, ks = n % KSTEPS;
+          sn[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              fr[n % AHEAD], qf[ks], ks ? sn[t] : f32x16v{}, 0, 0, 0);
+        } else {
+          const int t = (n - NS) % DT, ks = (n - NS) / DT;
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              fr[n % AHEAD], __builtin_bit_cast(bf16x8v, w[ks]), o[t], 0, 0, 0);
+        }
+        if (n + AHEAD < NM) load(n + AHEAD);
+        // 16 pairs of weights; each slice of four comes before its first product
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+          if (u * (NM - 4) / 16 == n) w[u / 4][u % 4] = weigh(sp, u / 4, u % 4);
+        if constexpr (!FP8) {
+          if (n < KPER) copy_k(Kn, n);
+          else if (n - KPER < VPER) copy_v(Vn, n - KPER);
+          else if (n == KPER + VPER) pages(min(kt + 2, k1 - 1), min(kt + 1, k1 - 1));
+        }
+        if (n == NS) mx = larger(sn[0][0], sn[0]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      mx = top_of(larger(mx, sn[1]));
+      l += lsum;
+      lsum = 0.f;
+      if constexpr (FP8) {
+        settle_k(Kn);
+        settle_v(Vn);
+      }
+    };
+
+    const int whole = max(max(k0 + 1, (lo_least + SP_KT - 1) / SP_KT + 1),
+                          (lo_most + SP_KT - 1) / SP_KT);
+    const int cut = wave_on && a.softcap <= 0.f ? min(k1, P / SP_KT) : 0;
+
+    pages(k0, k0);
+    if constexpr (FP8) {
+      fetch_k();
+      settle_k(K0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < KPER; ++i) copy_k(K0, i);
+    }
+    pages(min(k0 + 1, k1 - 1), k0);
+    for (int kt = k0; kt <= k1; kt += 2) {
+      for (; kt >= whole && kt + 1 < cut; kt += 2) {
+        whole_turn(kt, K0, K1, V1, V0, s1, s0);
+        whole_turn(kt + 1, K1, K0, V0, V1, s0, s1);
+      }
+      cut_turn(kt, K0, K1, V1, V0);
+      if (kt + 1 <= k1) cut_turn(kt + 1, K1, K0, V0, V1);
     }
 
     l = over_halves(l, [](float x, float y) { return x + y; });
@@ -431,12 +520,12 @@ DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
     todo -= k1 - k0;
     done += k1 - k0;
     at += k1 - k0;
-    const int tiles = tiles_of(g);
+    const int tiles = w.tiles(g, G);
     if (at == tiles * keys) {
       at = 0;
       tile0 += tiles;
       do ++g;
-      while (g < a.N && count[g] == 0);
+      while (g < a.N && w.count[g] == 0);
       g = uniform(g);
     }
   }
@@ -445,9 +534,9 @@ DEVINL void prefix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
 // ---- suffixes ----------------------------------------------------------------------
 
 template <int D, bool FP8>
-DEVINL void suffix_role(const SharedPrefix& a, uint8_t* S, const int hk, const int run) {
-  constexpr int W = 4;
-  constexpr int KT = 32;                 // tokens a tile
+DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const int hk,
+                        const int run, const int total, const int runs) {
+  constexpr int KT = SP_UNIT;
   constexpr int ES = FP8 ? 1 : 2;
   constexpr int RB = D * ES;             // bytes a K row
   constexpr int CPR = RB / 16;
@@ -456,10 +545,7 @@ DEVINL void suffix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
   constexpr int NC = TILE / 1024;        // copies of K, and of V
   constexpr int KC = D / 32;
   constexpr int MT = D / 16;
-  constexpr int U = SP_UNIT;
-  constexpr int MROW = D + 4;            // floats a row where sums are added
-  static_assert(W * KT == U && W * 2 * TILE <= tiles_bytes(D) &&
-                W * 16 * MROW * 4 <= tiles_bytes(D) && SP_ROWS * 4 <= tiles_bytes(D), "");
+  static_assert(4 * 2 * TILE <= tiles_bytes(D) && SP_ROWS * 4 <= tiles_bytes(D), "");
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wid = uniform(tid >> 6);
@@ -467,46 +553,26 @@ DEVINL void suffix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
   const int l4 = lane >> 4;
   const int G = a.Hq / a.Hk, BS = 1 << a.shift;
 
-  float(*ms)[16] = (float(*)[16])(S + tiles_bytes(D));
-  float(*ls)[16] = ms + W;
-
-  // ---- this workgroup's run of units ------------------------------------------------
-  int* const units = (int*)S;  // of every row, before the tiles lie there
-  for (int b = tid; b < a.B; b += 256) {
-    const int L = a.lens[b];
-    units[b] = suffix_units(max(prefix_of(a, b), window_start(a, L)), L);
-  }
-  __syncthreads();
-  int seq = 0, at = 0, todo = 0, per = 1;
-  {
-    int total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64)
-      total += b0 + lane < a.B ? units[b0 + lane] : 0;
-    total = __shfl(scan64(total), 63, WAVE_SIZE);
-    per = max((total + a.s_runs - 1) / a.s_runs, 1);
-    const int begin = run * per;
-    if (begin >= total) return;
-    todo = min(per, total - begin);
-    int before = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int n = b0 + lane < a.B ? units[b0 + lane] : 0;
-      const int s = scan64(n);
-      const unsigned long long hit = __ballot(before + s > begin);
-      if (hit) {
-        const int src = __ffsll(hit) - 1;
-        seq = b0 + src;
-        at = begin - before - __shfl(s, src, WAVE_SIZE) + __shfl(n, src, WAVE_SIZE);
-        break;
-      }
-      before += __shfl(s, 63, WAVE_SIZE);
+  // ---- this wave's run of tiles --------------------------------------------------------
+  const int wave = run * 4 + wid;
+  const int per = max((total + 4 * runs - 1) / (4 * runs), 1);
+  const int begin = wave * per;
+  const int todo = uniform(max(0, min(per, total - begin)));
+  int seq = 0, at = 0, before = 0;
+  for (int b0 = 0; b0 < a.B && todo > 0; b0 += 64) {
+    const int n = b0 + lane < a.B ? w.units[b0 + lane] : 0;
+    const int s = scan64(n);
+    const unsigned long long hit = __ballot(before + s > begin);
+    if (hit) {
+      const int src = __ffsll(hit) - 1;
+      seq = b0 + src;
+      at = begin - before - __shfl(s, src, WAVE_SIZE) + __shfl(n, src, WAVE_SIZE);
+      break;
     }
+    before += __shfl(s, 63, WAVE_SIZE);
   }
   __syncthreads();  // the list is read
-  seq = uniform(seq);
-  at = uniform(at);
-  todo = uniform(todo);
-  per = uniform(per);
-  int done = 0;  // units of the run so far
+  if (todo == 0) return;
 
   uint8_t* Kt = S + wid * (2 * TILE);
   uint8_t* Vt = Kt + TILE;
@@ -527,223 +593,242 @@ DEVINL void suffix_role(const SharedPrefix& a, uint8_t* S, const int hk, const i
           : lds_at(Vt) + l15 * VB + (l4 ^ swz_v<FP8>(l15)) * 16;
   const float c = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1e-20f);
 
-  while (todo > 0) {
-    const int L = a.lens[seq];
-    const int P = prefix_of(a, seq);
-    const int lo = max(P, window_start(a, L));
-    const int units = suffix_units(lo, L);
-    if (at >= units) {  // a row without tokens of its own
-      ++seq;
-      at = 0;
-      continue;
-    }
-    const int t0 = at, t1 = min(units, at + todo);
-    if (t0 == 0 && hk == 0 && tid == 0)
-      a.s_info[seq] = make_int2(run, run + (done + units - 1) / per);
-    const int unit0 = lo / U;
+  // Rows 64 at a time, one a lane: where its own tokens begin and end.
+  int rows0 = -64, row_lo = 0, row_end = 0;
+  unsigned long long filled = 0, grouped = 0;
+  auto look = [&](int b0) INL {
+    rows0 = b0;
+    const int b = min(b0 + lane, a.B - 1);
+    const int g = a.group[b];
+    row_end = a.lens[b];
+    int P = g >= 0 && g < a.N ? w.prefix[g] : 0;
+    if (P <= 0 || row_end < P) P = 0;
+    row_lo = max(P, window_start(a, row_end));
+    grouped = __ballot(P > 0);
+    filled = __ballot(b0 + lane < a.B && row_lo < row_end);
+  };
+  // One tile after the other, across rows: while one is computed, the next is copied
+  // and the pages of the one behind that are looked up.
+  struct Tile {
+    int row, tok, lo, end;  // a row, the tile's first token, the row's own tokens
+    int p0, p1;             // pages of the tile's two halves
+    int grouped;
+  };
+  auto row_of = [&](Tile& t, int row) INL {
+    t.row = row;
+    t.lo = __builtin_amdgcn_readlane(row_lo, row - rows0);
+    t.end = __builtin_amdgcn_readlane(row_end, row - rows0);
+    t.grouped = (int)(grouped >> (row - rows0)) & 1;
+  };
+  auto pages = [&](Tile& t) INL {
+    // constant memory: read by the scalar unit, no vector load among the copies
     const auto* table = (const __attribute__((address_space(4))) int*)(
-        a.tables + (size_t)seq * a.max_blocks);
-
-    bf16x8v qf[KC];
-    {
-      const uint16_t* row = a.q + seq * a.q_stride + (hk * G + min(l15, G - 1)) * D;
-#pragma unroll
-      for (int s = 0; s < KC; ++s)
-        qf[s] = *(const bf16x8v*)(row + (FP8 ? ((s >> 1) * 4 + l4) * 16 + (s & 1) * 8
-                                             : s * 32 + l4 * 8));
-    }
-    f32x4v o[MT] = {};
-    float m = kLowest, l = 0.f;
-
-    // this wave's tiles: from first on, a unit apart
-    int first = (unit0 + t0) * U + wid * KT;
-    if (first + KT <= lo) first += U;
-    const int end = min(L, (unit0 + t1) * U);
-    // past the end the copies are of the last tile again: the count of copies in
-    // flight stays the same
-    const int last = (L - 1) & ~(KT - 1);
-    auto pages = [&](int tok, int(&p)[2]) INL {  // of the tile's two halves
-      const int x = min(tok, last);
-      p[0] = page_at(a, table[x >> a.shift]);
-      p[1] = page_at(a, table[min(a.shift == 4 ? x + 16 : x, L - 1) >> a.shift]);
-    };
-    auto issue_k = [&](int tok, const int(&p)[2]) INL {
-      const int64_t in = head_off + (int64_t)(min(tok, last) & (BS - 1)) * RB;
-      const uint8_t* b0 = a.k + p[0] * page_bytes + in;
-      const uint8_t* b1 = a.k + p[1] * page_bytes + in;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        constexpr int RC = 64 / CPR;  // rows a copy
-        const uint32_t off = k_row * RB + (k_ch ^ swz_k<CPR>(i * RC)) * 16;
-        // the second 16 rows: of the second page, if pages have 16
-        const uint8_t* b = i < NC / 2 ? b0 + i * 1024
-                           : a.shift == 4 ? b1 + (i - NC / 2) * 1024
-                                          : b0 + i * 1024;
-        copy16_to_lds(b + off, Kt + i * 1024);
+        a.tables + (size_t)t.row * a.max_blocks);
+    t.p0 = page_at(a, table[t.tok >> a.shift]);
+    t.p1 = page_at(a, table[min(a.shift == 4 ? t.tok + 16 : t.tok, t.end - 1) >> a.shift]);
+  };
+  auto next = [&](const Tile& t) INL {  // the same where no row has one
+    Tile n = t;
+    n.tok += KT;
+    if (n.tok >= t.end) {
+      unsigned long long rest =
+          t.row >= rows0 + 63 ? 0 : filled & (~0ull << (t.row + 1 - rows0));
+      while (rest == 0 && rows0 + 64 < a.B) {
+        look(rows0 + 64);
+        rest = filled;
       }
-    };
-    auto issue_v = [&](int tok, const int(&p)[2]) INL {
-      const int64_t in = head_off + (int64_t)(min(tok, last) & (BS - 1)) * ES;
-      const int64_t page = v_second ? p[1] : p[0];
-      const uint8_t* b = a.v + in + page * page_bytes + v_off;
-#pragma unroll
-      for (int i = 0; i < NC; ++i)
-        copy16_to_lds(b + i * (1024 / VB) * BS * ES, Vt + i * 1024);
-    };
-
-    if (first < end) {
-      int nx[2];
-      pages(first, nx);
-      issue_k(first, nx);
-      issue_v(first, nx);
-      pages(first + U, nx);
-      if (a.scale < 0.f) {  // the sign goes with q, as c takes maxima
-#pragma unroll
-        for (int s = 0; s < KC; ++s)
-          qf[s] = __builtin_bit_cast(
-              bf16x8v, __builtin_bit_cast(u32x4v, qf[s]) ^ 0x80008000u);
-      }
-      for (int tok = first; tok < end; tok += U) {
-        wait_copies<NC>();
-        u32x4v kr[KC * ES];  // [chunk group][t]
-        if constexpr (CPR == 16)
-          read8<4 * RB>(kr, k_at, k_at ^ 64, k_at ^ 128, k_at ^ 192);
-        else if constexpr (CPR == 8)
-          read4<4 * RB>(kr, k_at, k_at ^ 64);
-        else
-          read2<4 * RB>(kr, k_at);
-        issue_k(tok + U, nx);
-
-        // token of s[t][r]: tok + 8 l4 + 4 t + r
-        f32x4v s[2] = {};
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int k = 0; k < KC; ++k) {
-            bf16x8v x;
-            if constexpr (FP8) {
-              const u32x4v r = kr[(k >> 1) * 2 + t];
-              x = k & 1 ? widen(r[2], r[3]) : widen(r[0], r[1]);
-            } else {
-              x = __builtin_bit_cast(bf16x8v, kr[k * 2 + t]);
-            }
-            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qf[k], s[t], 0, 0, 0);
-          }
-        if (a.softcap > 0.f) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            s[e >> 2][e & 3] = a.softcap *
-                               tanhf(s[e >> 2][e & 3] * fabsf(a.scale) / a.softcap) *
-                               kLog2e;
-        }
-        const bool cut = tok + KT > L || tok < lo;
-        if (cut) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int k = tok + 8 * l4 + e;
-            s[e >> 2][e & 3] = k >= lo && k < L ? s[e >> 2][e & 3] : kHidden;
-          }
-        }
-        float mx = s[0][0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
-        mx = over_head(mx, [](float x, float y) { return fmaxf(x, y); }) * c;
-        if (__any(mx > m)) {
-          const float m2 = fmaxf(m, mx);
-          const float f = __builtin_amdgcn_exp2f(m - m2);
-          m = m2;
-          l *= f;
-#pragma unroll
-          for (int t = 0; t < MT; ++t) o[t] *= f;
-        }
-        u32x4v pk;
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], c, -m));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][(e & 3) + 1], c, -m));
-          l += p0 + p1;
-          pk[e >> 1] = pack_bf16(p0, p1);
-        }
-
-        wait_copies<NC>();
-        using VR = std::conditional_t<FP8, u32x2v, u32x4v>;
-        VR vr[MT];
-        read_rows(vr, v_at);
-        issue_v(tok + U, nx);
-        pages(tok + 2 * U, nx);
-        // slots past the end, and before the row's own tokens, may hold anything:
-        // weight 0 times it
-        u32x4v keep = {~0u, ~0u, ~0u, ~0u};
-        if (cut) {
-          const int from = lo - tok - 8 * l4, to = L - tok - 8 * l4;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            keep[i] = (2 * i >= from && 2 * i < to ? 0xffffu : 0u) |
-                      (2 * i + 1 >= from && 2 * i + 1 < to ? 0xffff0000u : 0u);
-        }
-        const bf16x8v pb = __builtin_bit_cast(bf16x8v, pk);
-#pragma unroll
-        for (int d = 0; d < MT; ++d) {
-          u32x4v x;
-          if constexpr (FP8)
-            x = __builtin_bit_cast(u32x4v, widen(vr[d][0], vr[d][1]));
-          else
-            x = vr[d];
-          if (cut) x &= keep;
-          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(bf16x8v, x), pb, o[d], 0, 0, 0);
-        }
-      }
-      wait_copies<0>();
+      if (rest == 0) return t;
+      row_of(n, rows0 + __ffsll(rest) - 1);
+      n.tok = n.lo & ~(KT - 1);
     }
-
-    // ---- the waves' sums -------------------------------------------------------------
-    l = over_head(l, [](float x, float y) { return x + y; });
-    if (l4 == 0) {
-      ms[wid][l15] = m;
-      ls[wid][l15] = l;
+    pages(n);
+    return n;
+  };
+  auto issue_k = [&](const Tile& t) INL {
+    const int64_t in = head_off + (int64_t)(t.tok & (BS - 1)) * RB;
+    const uint8_t* b0 = a.k + t.p0 * page_bytes + in;
+    const uint8_t* b1 = a.k + t.p1 * page_bytes + in;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      constexpr int RC = 64 / CPR;  // rows a copy
+      const uint32_t off = k_row * RB + (k_ch ^ swz_k<CPR>(i * RC)) * 16;
+      // the second 16 rows: of the second page, if pages have 16
+      const uint8_t* b = i < NC / 2 ? b0 + i * 1024
+                         : a.shift == 4 ? b1 + (i - NC / 2) * 1024
+                                        : b0 + i * 1024;
+      copy16_to_lds(b + off, Kt + i * 1024);
     }
-    __syncthreads();
-    float M = kLowest;
+  };
+  auto issue_v = [&](const Tile& t) INL {
+    const int64_t in = head_off + (int64_t)(t.tok & (BS - 1)) * ES;
+    const int64_t page = v_second ? t.p1 : t.p0;
+    const uint8_t* b = a.v + in + page * page_bytes + v_off;
 #pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, ms[w][l15]);
-    const float f = __builtin_amdgcn_exp2f(m - M);
-    float* sums = reinterpret_cast<float*>(S);
+    for (int i = 0; i < NC; ++i)
+      copy16_to_lds(b + i * (1024 / VB) * BS * ES, Vt + i * 1024);
+  };
+  bf16x8v qf[KC];
+  auto load_q = [&](int row) INL {
+    const uint16_t* src = a.q + row * a.q_stride + (hk * G + min(l15, G - 1)) * D;
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-      *reinterpret_cast<f32x4v*>(sums + (wid * 16 + l15) * MROW + t * 16 + l4 * 4) =
-          o[t] * f;
-    __syncthreads();
-    const bool whole = P == 0 && t0 == 0 && t1 == units;
-    for (int e = tid; e < G * (D / 4); e += W * 64) {
-      const int g = e / (D / 4), d = e % (D / 4) * 4;
-      float Mg = kLowest, lg = 0.f;
+    for (int s = 0; s < KC; ++s)
+      qf[s] = *(const bf16x8v*)(src + (FP8 ? ((s >> 1) * 4 + l4) * 16 + (s & 1) * 8
+                                           : s * 32 + l4 * 8));
+  };
+
+  const float sink = a.sinks != nullptr ? a.sinks[hk * G + min(l15, G - 1)] * kLog2e
+                                        : kHidden;
+  seq = uniform(seq);
+  look(seq & ~63);
+  Tile t0 = {};
+  row_of(t0, seq);
+  t0.tok = (t0.lo & ~(KT - 1)) + uniform(at) * KT;
+  pages(t0);
+  load_q(t0.row);
+  issue_k(t0);
+  issue_v(t0);
+  // past the run the copies are of its last tile again: the count of copies in flight
+  // stays the same
+  Tile t1 = todo > 1 ? next(t0) : t0;
+  int from = t0.tok;  // this wave's first token of the row
+  f32x4v o[MT] = {};
+  float m = kLowest, l = 0.f;
+
+  for (int i = 0; i < todo; ++i) {
+    const int tok = t0.tok, lo = t0.lo, L = t0.end;
+    if (tok <= lo && hk == 0 && lane == 0)  // a row's first tile
+      a.s_info[t0.row] =
+          make_int2(wave, wave + (i + suffix_units(lo, L) - 1) / per);
+    wait_copies<NC>();
+    u32x4v kr[KC * ES];  // [chunk group][t]
+    if constexpr (CPR == 16)
+      read8<4 * RB>(kr, k_at, k_at ^ 64, k_at ^ 128, k_at ^ 192);
+    else if constexpr (CPR == 8)
+      read4<4 * RB>(kr, k_at, k_at ^ 64);
+    else
+      read2<4 * RB>(kr, k_at);
+    issue_k(t1);
+
+    // token of s[t][r]: tok + 8 l4 + 4 t + r
+    f32x4v s[2] = {};
 #pragma unroll
-      for (int w = 0; w < W; ++w) Mg = fmaxf(Mg, ms[w][g]);
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int w = 0; w < W; ++w) lg += ls[w][g] * __builtin_amdgcn_exp2f(ms[w][g] - Mg);
-      f32x4v s = {};
+      for (int k = 0; k < KC; ++k) {
+        bf16x8v x;
+        if constexpr (FP8) {
+          const u32x4v r = kr[(k >> 1) * 2 + t];
+          x = k & 1 ? widen(r[2], r[3]) : widen(r[0], r[1]);
+        } else {
+          x = __builtin_bit_cast(bf16x8v, kr[k * 2 + t]);
+        }
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qf[k], s[t], 0, 0, 0);
+      }
+    if (a.scale < 0.f) {  // maxima are taken of the scores of -q
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-        s += *reinterpret_cast<const f32x4v*>(sums + (w * 16 + g) * MROW + d);
-      const int h = hk * G + g;
-      if (whole) {
-        if (a.sinks != nullptr) lg += __builtin_amdgcn_exp2f(a.sinks[h] * kLog2e - Mg);
-        s *= a.v_scale / lg;
-        *reinterpret_cast<uint2*>(a.out + ((int64_t)seq * a.Hq + h) * D + d) =
-            make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
-      } else {
-        const int64_t part = (int64_t)(run + seq) * a.Hq + h;
-        *reinterpret_cast<f32x4v*>(a.s_acc + part * D + d) = s;
-        if (d == 0) *reinterpret_cast<f32x2v*>(a.s_ml + part * 2) = f32x2v{Mg, lg};
+      for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] = -s[e >> 2][e & 3];
+    }
+    if (a.softcap > 0.f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        s[e >> 2][e & 3] = a.softcap *
+                           tanhf(s[e >> 2][e & 3] * fabsf(a.scale) / a.softcap) *
+                           kLog2e;
+    }
+    const bool cut = tok + KT > L || tok < lo;
+    if (cut) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int k = tok + 8 * l4 + e;
+        s[e >> 2][e & 3] = k >= lo && k < L ? s[e >> 2][e & 3] : kHidden;
       }
     }
-    __syncthreads();
-    todo -= t1 - t0;
-    done += t1 - t0;
-    ++seq;
-    at = 0;
+    float mx = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
+    mx = over_head(mx, [](float x, float y) { return fmaxf(x, y); }) * c;
+    if (__any(mx > m)) {
+      const float m2 = fmaxf(m, mx);
+      const float f = __builtin_amdgcn_exp2f(m - m2);
+      m = m2;
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) o[t] *= f;
+    }
+    u32x4v pk;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], c, -m));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][(e & 3) + 1], c, -m));
+      l += p0 + p1;
+      pk[e >> 1] = pack_bf16(p0, p1);
+    }
+    // Not right behind the products: where paths meet there, one of them without
+    // instructions, the compiler leaves out the wait for their results (seen in what it
+    // wrote, and in the last score of four).
+    if (t1.row != t0.row) load_q(t1.row);
+
+    wait_copies<NC>();
+    using VR = std::conditional_t<FP8, u32x2v, u32x4v>;
+    VR vr[MT];
+    read_rows(vr, v_at);
+    issue_v(t1);
+    const Tile t2 = i + 2 < todo ? next(t1) : t1;
+    // slots past the end, and before the row's own tokens, may hold anything:
+    // weight 0 times it
+    u32x4v keep = {~0u, ~0u, ~0u, ~0u};
+    if (cut) {
+      const int first = lo - tok - 8 * l4, end = L - tok - 8 * l4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        keep[j] = (2 * j >= first && 2 * j < end ? 0xffffu : 0u) |
+                  (2 * j + 1 >= first && 2 * j + 1 < end ? 0xffff0000u : 0u);
+    }
+    const bf16x8v pb = __builtin_bit_cast(bf16x8v, pk);
+#pragma unroll
+    for (int d = 0; d < MT; ++d) {
+      u32x4v x;
+      if constexpr (FP8)
+        x = __builtin_bit_cast(u32x4v, widen(vr[d][0], vr[d][1]));
+      else
+        x = vr[d];
+      if (cut) x &= keep;
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+          __builtin_bit_cast(bf16x8v, x), pb, o[d], 0, 0, 0);
+    }
+
+    // ---- out: column l15 = head, rows of O^T = d -----------------------------------------
+    if (t1.row != t0.row || i + 1 == todo) {
+      l = over_head(l, [](float x, float y) { return x + y; });
+      if (l15 < G) {
+        const int h = hk * G + l15;
+        if (!t0.grouped && from <= lo && tok + KT >= L) {  // all that it sees
+          l += __builtin_amdgcn_exp2f(sink - m);
+          const float f = a.v_scale / l;
+          uint16_t* dst = a.out + ((int64_t)t0.row * a.Hq + h) * D + l4 * 4;
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+            *reinterpret_cast<uint2*>(dst + t * 16) =
+                make_uint2(pack_bf16(o[t][0] * f, o[t][1] * f),
+                           pack_bf16(o[t][2] * f, o[t][3] * f));
+        } else {
+          const int64_t part = (int64_t)(wave + t0.row) * a.Hq + h;
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+            *reinterpret_cast<f32x4v*>(a.s_acc + part * D + t * 16 + l4 * 4) = o[t];
+          if (l4 == 0) *reinterpret_cast<f32x2v*>(a.s_ml + part * 2) = f32x2v{m, l};
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) o[t] = f32x4v{};
+      m = kLowest;
+      l = 0.f;
+      from = t1.tok;
+    }
+    t0 = t1;
+    t1 = t2;
   }
+  wait_copies<0>();
 }
 
 }  // namespace
@@ -753,8 +838,57 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(
     const SharedPrefix a) {
   __shared__ __attribute__((aligned(1024))) uint8_t S[lds_bytes(D)];
   const int hk = blockIdx.x % a.Hk, run = blockIdx.x / a.Hk;
-  if (run < a.p_runs) prefix_role<D, FP8>(a, S, hk, run);
-  else suffix_role<D, FP8>(a, S, hk, run - a.p_runs);
+  const int tid = threadIdx.x, lane = tid & 63;
+  Lists w;
+  w.units = (int*)S;
+  w.prefix = (int*)(S + tiles_bytes(D));
+  w.count = w.prefix + SP_GROUPS;
+  w.low = w.count + SP_GROUPS;
+  w.rows = w.low + SP_GROUPS;
+  w.member = (int16_t*)(w.rows + SP_ITEMS + 4);
+  int* const sum = w.rows;  // of all units
+  for (int g = tid; g < a.N; g += 256) {
+    w.prefix[g] = a.prefix[g];
+    w.count[g] = 0;
+    w.low[g] = INT_MAX;
+  }
+  if (tid == 0) *sum = 0;
+  __syncthreads();
+  int mine = 0;
+  for (int b = tid; b < a.B; b += 256) {
+    const int L = a.lens[b], g = a.group[b];
+    int P = g >= 0 && g < a.N ? w.prefix[g] : 0;
+    if (P <= 0 || L < P) P = 0;
+    const int lo = window_start(a, L);
+    w.member[b] = (int16_t)(P > 0 ? g : -1);
+    if (P > 0) {
+      atomicAdd(w.count + g, 1);
+      atomicMin(w.low + g, lo);
+    }
+    const int n = suffix_units(max(P, lo), L);
+    w.units[b] = n;
+    mine += n;
+  }
+  mine = __shfl(scan64(mine), 63, WAVE_SIZE);
+  if (lane == 0) atomicAdd(sum, mine);
+  __syncthreads();
+  const int s_total = uniform(*sum);
+  int p_total = 0;
+  for (int g0 = 0; g0 < a.N; g0 += 64) {
+    const int g = g0 + lane;
+    int kb, n = 0;
+    if (g < a.N && w.count[g] > 0) n = w.tiles(g, a.Hq / a.Hk) * (w.keys(g, &kb) - kb);
+    p_total += __shfl(scan64(n), 63, WAVE_SIZE);
+  }
+  p_total = uniform(p_total);
+  __syncthreads();  // the sum is read
+  const float p_cost = p_total, s_cost = s_total * a.ratio;
+  int p_runs = (int)(a.runs * (p_cost / (p_cost + s_cost)) + 0.5f);
+  p_runs = p_total == 0 ? 0 : s_total == 0 ? a.runs : min(max(p_runs, 1), a.runs - 1);
+  if (run < p_runs)
+    prefix_role<D, FP8>(a, w, S, hk, run, p_total, p_runs);
+  else
+    suffix_role<D, FP8>(a, w, S, hk, run - p_runs, s_total, a.runs - p_runs);
 }
 
 // Joins the parts of every row and query head: a wave each. Lanes take a part each for
@@ -776,7 +910,7 @@ __global__ __launch_bounds__(256) void shared_prefix_join_kernel(const SharedPre
   }
   int2 sr = make_int2(0, -1);
   if (su > 0) sr = a.s_info[b];
-  if (P == 0 && sr.x == sr.y) return;  // finished by its run
+  if (P == 0 && sr.x == sr.y) return;  // finished by its wave
   int4 pi = make_int4(0, 0, 0, 0);
   if (P > 0) pi = a.p_info[(int64_t)b * a.Hq + h];
   const int np = pi.y, parts = np + sr.y - sr.x + 1;
@@ -823,18 +957,21 @@ __global__ __launch_bounds__(256) void shared_prefix_join_kernel(const SharedPre
         make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
 }
 
-// Workgroups of a key/value head for prefixes and for suffixes, and the item tiles that
-// B rows of N groups make at most.
-extern "C" void shared_prefix_plan(int B, int N, int Hq, int Hk, int D, int* p_runs,
-                                   int* s_runs, int* tiles) {
-  const int slots = std::max(1, (D == 128 ? 256 : 512) / Hk);
-  *p_runs = N > 0 ? slots : 0;
-  *s_runs = slots;
+// Workgroups of a key/value head, and the item tiles that B rows of N groups make at
+// most.
+extern "C" void shared_prefix_plan(int B, int N, int Hq, int Hk, int D, int* runs,
+                                   int* tiles) {
+  const char* e = getenv("SP_P");
+  *runs = std::max(2, (e && atoi(e) ? atoi(e) : D == 128 ? 512 : 768) / Hk);
   *tiles = N > 0 ? (int)((int64_t)B * (Hq / Hk) / SP_ITEMS) + std::min(N, B) : 0;
 }
 
-extern "C" void launch_shared_prefix(const SharedPrefix* a, bool fp8, hipStream_t stream) {
-  const dim3 grid((a->p_runs + a->s_runs) * a->Hk);
+extern "C" void launch_shared_prefix(const SharedPrefix* a_, bool fp8, hipStream_t stream) {
+  SharedPrefix a2 = *a_;
+  SharedPrefix* a = &a2;
+  const char* e = getenv("SP_S");
+  a2.ratio = e ? atof(e) : 2.f;
+  const dim3 grid(a->runs * a->Hk);
   auto run = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(*a); };
   if (a->D == 128) fp8 ? run(shared_prefix_kernel<128, true>)
                        : run(shared_prefix_kernel<128, false>);
