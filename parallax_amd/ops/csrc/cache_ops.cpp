@@ -47,6 +47,7 @@ struct SharedPrefix {
   int4* p_info;
   float *s_acc, *s_ml;
   int2* s_info;
+  int* has;
 };
 
 extern "C" {
@@ -249,7 +250,7 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   // parts lie
   const int64_t p_items = N > 0 ? (int64_t)(a.runs + tiles) * Hk * 128 : 0;
   const int64_t s_items = (4 * a.runs + B) * Hq;
-  const int64_t words = (p_items + s_items) * (D + 2) + B * Hq * 4 + B * 2;
+  const int64_t words = (p_items + s_items) * (D + 2) + B * Hq * 4 + B * 3;
   auto work = torch::empty({words}, q.options().dtype(at::kFloat));
   float* at = work.data_ptr<float>();
   auto take = [&](int64_t n) { return std::exchange(at, at + n); };
@@ -259,6 +260,7 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   a.p_ml = take(p_items * 2);
   a.s_ml = take(s_items * 2);
   a.s_info = (int2*)take(B * 2);
+  a.has = (int*)take(B);
   launch_shared_prefix(&a, fp8, stream());
   return out;
 }

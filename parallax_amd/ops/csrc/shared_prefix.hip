@@ -28,6 +28,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstdlib>
+#include <type_traits>
 
 #include "common.h"
 #include "decode_common.h"
@@ -59,6 +60,7 @@ struct SharedPrefix {
   float* s_acc;  // [s_parts, Hq, D]: part wave + row
   float* s_ml;   // [s_parts, Hq, 2]
   int2* s_info;  // [B]: first and last wave; rows with tokens behind a prefix only
+  int* has;      // [B]: 1: of a prefix, + 2: behind one
 };
 
 namespace {
@@ -79,6 +81,18 @@ DEVINL int suffix_units(int lo, int L) {
 }
 
 DEVINL int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+DEVINL int of_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+
+// inclusive sum over the lanes of a wave, without LDS
+DEVINL int sum_to_lane(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // of the row: 1 before
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // of the row before
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // of both before
+  return v;
+}
 
 DEVINL int page_at(const SharedPrefix& a, int entry) {
   return min(max(entry, 0), a.num_pages - 1);
@@ -149,21 +163,18 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       t = w.tiles(x, G);
       n = t * (w.keys(x, &kb) - kb);
     }
-    const int ns = scan64(n), ts = scan64(t);
+    const int ns = sum_to_lane(n), ts = sum_to_lane(t);
     const unsigned long long hit = __ballot(before + ns > begin);
     if (hit) {
       const int src = __ffsll(hit) - 1;
       g = g0 + src;
-      at = begin - before - __shfl(ns, src, WAVE_SIZE) + __shfl(n, src, WAVE_SIZE);
-      tile0 += __shfl(ts, src, WAVE_SIZE) - __shfl(t, src, WAVE_SIZE);
+      at = begin - before - of_lane(ns, src) + of_lane(n, src);
+      tile0 += of_lane(ts, src) - of_lane(t, src);
       break;
     }
-    before += __shfl(ns, 63, WAVE_SIZE);
-    tile0 += __shfl(ts, 63, WAVE_SIZE);
+    before += of_lane(ns, 63);
+    tile0 += of_lane(ts, 63);
   }
-  g = uniform(g);
-  at = uniform(at);
-  tile0 = uniform(tile0);
 
   // ---- what a lane copies and reads -------------------------------------------------
   // 16 chunks (256 bytes) make a turn over the banks: a K row of 128 values, or two of
@@ -195,7 +206,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
 
   int done = 0;
   while (todo > 0) {
-    const int n_items = w.count[g] * G;
+    const int n_items = uniform(w.count[g]) * G;
     const int P = uniform(w.prefix[g]);
     int kb;
     const int kend = uniform(w.keys(g, &kb));
@@ -225,17 +236,19 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     const int r = min(item, n_items - 1) / G;
     const int row = w.rows[r - r0];
     const int h = hk * G + min(item, n_items - 1) - r * G;
-    const int lo = window_start(a, a.lens[row]);
+    const int lo = a.window > 0 ? window_start(a, a.lens[row]) : 0;
     // constant memory: read by the scalar unit
     const auto* table = (const __attribute__((address_space(4))) int*)(
         a.tables + (size_t)uniform(w.rows[SP_ITEMS]) * a.max_blocks);
     const bool wave_on = tile * SP_ITEMS + wid * 32 < n_items;
     int lo_most = lo;
+    if (a.window > 0) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1)
-      lo_most = max(lo_most, __shfl_xor(lo_most, o, WAVE_SIZE));
+      for (int o = 1; o < 32; o <<= 1)
+        lo_most = max(lo_most, __shfl_xor(lo_most, o, WAVE_SIZE));
+    }
     lo_most = uniform(lo_most);
-    const int lo_least = w.low[g];
+    const int lo_least = uniform(w.low[g]);
 
     if (k0 == kb && half == 0 && on)
       a.p_info[(int64_t)row * a.Hq + h] =
@@ -331,22 +344,28 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
           for (int e = 0; e < 16; ++e) o[t][e] *= f;
       }
     };
-    auto meet = [&]() INL {  // all copies and stores to LDS, of all waves
+    // All copies and stores to LDS, of all waves; but those of this thread that may be
+    // under way.
+    auto meet = [&](auto left) INL {
+      constexpr int n = decltype(left)::value;
       asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0x0070);
+      __builtin_amdgcn_s_waitcnt(0x0070 | n);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     };
+    using none = std::integral_constant<int, 0>;
 
     // A turn takes the scores of tile kt and the weights and values of the tile before,
     // which depend on nothing of this turn. Any turn: also the first and the last, a
     // softcap, a mask.
     auto cut_turn = [&](int kt, const uint16_t* Kl, uint16_t* Kn, const uint16_t* Vl,
                         uint16_t* Vn) INL {
-      meet();
-      const bool more = kt < k1;
+      const bool more = kt < k1, first = kt == k0;
+      if (first) meet(std::integral_constant<int, FP8 ? 0 : KPER + VPER>{});
+      else meet(none{});
       if (more) {  // past the last tile K's copy is the last again
-        if constexpr (FP8) {
+        if (first) {
+        } else if constexpr (FP8) {
           fetch_k();
           fetch_v();
         } else {
@@ -420,7 +439,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       if constexpr (FP8)
         if (more) {
           settle_k(Kn);
-          settle_v(Vn);
+          if (!first) settle_v(Vn);
         }
     };
 
@@ -429,7 +448,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     // instructions early; the compiler's own puts every read right before its use.
     auto whole_turn = [&](int kt, const uint16_t* Kl, uint16_t* Kn, const uint16_t* Vl,
                           uint16_t* Vn, f32x16v(&sn)[2], const f32x16v(&sp)[2]) INL {
-      meet();
+      meet(none{});
       raise();
       constexpr int NS = 2 * KSTEPS, NM = NS + 4 * DT, AHEAD = 4;
       bf16x8v fr[AHEAD];
@@ -483,15 +502,28 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
                           (lo_most + SP_KT - 1) / SP_KT);
     const int cut = wave_on && a.softcap <= 0.f ? min(k1, P / SP_KT) : 0;
 
+    // The first turn's K, and behind it what that turn would ask for: the buffers are
+    // free, and short prefixes are rows of such waits.
     pages(k0, k0);
+    const int second = page_at(a, table[min(min(k0 + 1, k1 - 1) * SP_KT + wid * 16, P - 1) >>
+                                        a.shift]);
     if constexpr (FP8) {
       fetch_k();
+      fetch_v();
       settle_k(K0);
+      kpage = second;
+      fetch_k();
+      settle_v(V0);
     } else {
 #pragma unroll
       for (int i = 0; i < KPER; ++i) copy_k(K0, i);
+      asm volatile("" ::: "memory");
+      kpage = second;
+#pragma unroll
+      for (int i = 0; i < KPER; ++i) copy_k(K1, i);
+#pragma unroll
+      for (int i = 0; i < VPER; ++i) copy_v(V0, i);
     }
-    pages(min(k0 + 1, k1 - 1), k0);
     for (int kt = k0; kt <= k1; kt += 2) {
       for (; kt >= whole && kt + 1 < cut; kt += 2) {
         whole_turn(kt, K0, K1, V1, V0, s1, s0);
@@ -520,7 +552,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     todo -= k1 - k0;
     done += k1 - k0;
     at += k1 - k0;
-    const int tiles = w.tiles(g, G);
+    const int tiles = uniform(w.tiles(g, G));
     if (at == tiles * keys) {
       at = 0;
       tile0 += tiles;
@@ -561,15 +593,15 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   int seq = 0, at = 0, before = 0;
   for (int b0 = 0; b0 < a.B && todo > 0; b0 += 64) {
     const int n = b0 + lane < a.B ? w.units[b0 + lane] : 0;
-    const int s = scan64(n);
+    const int s = sum_to_lane(n);
     const unsigned long long hit = __ballot(before + s > begin);
     if (hit) {
       const int src = __ffsll(hit) - 1;
       seq = b0 + src;
-      at = begin - before - __shfl(s, src, WAVE_SIZE) + __shfl(n, src, WAVE_SIZE);
+      at = begin - before - of_lane(s, src) + of_lane(n, src);
       break;
     }
-    before += __shfl(s, 63, WAVE_SIZE);
+    before += of_lane(s, 63);
   }
   __syncthreads();  // the list is read
   if (todo == 0) return;
@@ -678,11 +710,10 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
 
   const float sink = a.sinks != nullptr ? a.sinks[hk * G + min(l15, G - 1)] * kLog2e
                                         : kHidden;
-  seq = uniform(seq);
   look(seq & ~63);
   Tile t0 = {};
   row_of(t0, seq);
-  t0.tok = (t0.lo & ~(KT - 1)) + uniform(at) * KT;
+  t0.tok = (t0.lo & ~(KT - 1)) + at * KT;
   pages(t0);
   load_q(t0.row);
   issue_k(t0);
@@ -868,9 +899,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(
     const int n = suffix_units(max(P, lo), L);
     w.units[b] = n;
     mine += n;
+    if (blockIdx.x == 0) a.has[b] = (P > 0) + 2 * (n > 0);
   }
-  mine = __shfl(scan64(mine), 63, WAVE_SIZE);
-  if (lane == 0) atomicAdd(sum, mine);
+  mine = sum_to_lane(mine);
+  if (lane == 63) atomicAdd(sum, mine);
   __syncthreads();
   const int s_total = uniform(*sum);
   int p_total = 0;
@@ -878,9 +910,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(
     const int g = g0 + lane;
     int kb, n = 0;
     if (g < a.N && w.count[g] > 0) n = w.tiles(g, a.Hq / a.Hk) * (w.keys(g, &kb) - kb);
-    p_total += __shfl(scan64(n), 63, WAVE_SIZE);
+    p_total += of_lane(sum_to_lane(n), 63);
   }
-  p_total = uniform(p_total);
   __syncthreads();  // the sum is read
   const float p_cost = p_total, s_cost = s_total * a.ratio;
   int p_runs = (int)(a.runs * (p_cost / (p_cost + s_cost)) + 0.5f);
@@ -891,65 +922,81 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(
     suffix_role<D, FP8>(a, w, S, hk, run - p_runs, s_total, a.runs - p_runs);
 }
 
-// Joins the parts of every row and query head: a wave each. Lanes take a part each for
-// the weights, then groups of D / 4 lanes the parts in turn, in a fixed order.
-template <int D>
+// Joins the parts of every row and query head, W waves each. A lane takes a part for
+// the weights; groups of D / 4 lanes take the parts in turn, in a fixed order.
+template <int D, int W>
 __global__ __launch_bounds__(256) void shared_prefix_join_kernel(const SharedPrefix a) {
-  const int lane = threadIdx.x & 63;
-  const int h = blockIdx.x * 4 + (threadIdx.x >> 6), b = blockIdx.y;
+  constexpr int Q = D / 4, GROUPS = 64 / Q, AHEAD = 4;
+  __shared__ f32x4v sums[W > 1 ? W : 1][Q];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int h = W > 1 ? blockIdx.x : blockIdx.x * 4 + wid, b = blockIdx.y;
   if (h >= a.Hq) return;
-  const int G = a.Hq / a.Hk, hk = h / G;
-  const int L = a.lens[b], P = prefix_of(a, b);
-  constexpr int Q = D / 4, GROUPS = 64 / Q;
+  const int wv = W > 1 ? wid : 0;
+  const int hk = h / (a.Hq / a.Hk);
   const int d = lane % Q * 4, grp = lane / Q;
+  // asked for together: what is not there is not looked at
+  const int has = a.has[b];
+  int4 pi = a.p_info[(int64_t)b * a.Hq + h];
+  int2 sr = a.s_info[b];
   uint16_t* out = a.out + ((int64_t)b * a.Hq + h) * D + d;
-  const int su = suffix_units(max(P, window_start(a, L)), L);
-  if (P == 0 && su == 0) {  // no tokens: zeros
-    if (grp == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
+  if (has == 0) {  // no tokens: zeros
+    if (wv == 0 && grp == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
     return;
   }
-  int2 sr = make_int2(0, -1);
-  if (su > 0) sr = a.s_info[b];
-  if (P == 0 && sr.x == sr.y) return;  // finished by its wave
-  int4 pi = make_int4(0, 0, 0, 0);
-  if (P > 0) pi = a.p_info[(int64_t)b * a.Hq + h];
+  if (!(has & 1)) pi = make_int4(0, 0, 0, 0);
+  if (!(has & 2)) sr = make_int2(0, -1);
+  if (has == 2 && sr.x == sr.y) return;  // finished by its wave
   const int np = pi.y, parts = np + sr.y - sr.x + 1;
-  // where part i lies
-  auto at = [&](int i, const float** ml, const float** acc) INL {
-    const int64_t x = i < np ? ((int64_t)(pi.x + i) * a.Hk + hk) * SP_ITEMS + pi.z
-                             : (int64_t)(sr.x + i - np + b) * a.Hq + h;
-    *ml = (i < np ? a.p_ml : a.s_ml) + x * 2;
-    *acc = (i < np ? a.p_acc : a.s_acc) + x * D;
+  // the place of part i
+  auto at = [&](int i) INL {
+    return i < np ? ((int64_t)(pi.x + i) * a.Hk + hk) * SP_ITEMS + pi.z
+                  : (int64_t)(sr.x + i - np + b) * a.Hq + h;
   };
+  auto load = [&](int i) INL {
+    return *reinterpret_cast<const f32x4v*>((i < np ? a.p_acc : a.s_acc) + at(i) * D + d);
+  };
+  const int first = wv * GROUPS + grp;
   float M = kLowest, l = 0.f;
   f32x4v s = {};
   for (int i0 = 0; i0 < parts; i0 += 64) {
-    const float *ml, *acc;
+    const int n = min(64, parts - i0);
+    f32x4v x[AHEAD];  // on their way while the weights are found
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) x[j] = load(i0 + min(first + j * W * GROUPS, n - 1));
     f32x2v v = {kLowest, 0.f};
-    if (i0 + lane < parts) {
-      at(i0 + lane, &ml, &acc);
-      v = *reinterpret_cast<const f32x2v*>(ml);
-    }
+    if (lane < n)
+      v = *reinterpret_cast<const f32x2v*>((i0 + lane < np ? a.p_ml : a.s_ml) +
+                                           at(i0 + lane) * 2);
     const float M2 = fmaxf(M, wave_reduce_max(v[0]));
     const float f = __builtin_amdgcn_exp2f(M - M2);
     const float w = __builtin_amdgcn_exp2f(v[0] - M2);
     M = M2;
     l = l * f + wave_reduce_sum(v[1] * w);
     s *= f;
-    const int n = min(64, parts - i0);
-#pragma unroll 4
-    for (int i = 0; i < n; i += GROUPS) {
-      const int mine = min(i + grp, n - 1);
-      const float x = __shfl(w, mine, WAVE_SIZE);
-      at(i0 + mine, &ml, &acc);
-      const f32x4v y = *reinterpret_cast<const f32x4v*>(acc + d);
-      s += y * (i + grp < n ? x : 0.f);
+    for (int j0 = 0; j0 < n; j0 += AHEAD * W * GROUPS) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int i = j0 + first + j * W * GROUPS;
+        const float y = __shfl(w, min(i, n - 1), WAVE_SIZE);
+        s += x[j] * (i < n ? y : 0.f);
+      }
+      if (j0 + AHEAD * W * GROUPS < n)
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+          x[j] = load(i0 + min(j0 + first + (AHEAD + j) * W * GROUPS, n - 1));
     }
   }
 #pragma unroll
   for (int o = Q; o < 64; o <<= 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += __shfl_xor(s[e], o, WAVE_SIZE);
+  if constexpr (W > 1) {
+    if (grp == 0) sums[wv][lane] = s;
+    __syncthreads();
+    if (wv > 0) return;
+#pragma unroll
+    for (int k = 1; k < W; ++k) s += sums[k][lane % Q];
+  }
   if (a.sinks != nullptr) l += __builtin_amdgcn_exp2f(a.sinks[h] * kLog2e - M);
   s *= a.v_scale / l;
   if (grp == 0)
@@ -970,13 +1017,18 @@ extern "C" void launch_shared_prefix(const SharedPrefix* a_, bool fp8, hipStream
   SharedPrefix a2 = *a_;
   SharedPrefix* a = &a2;
   const char* e = getenv("SP_S");
-  a2.ratio = e ? atof(e) : 2.f;
+  a2.ratio = e ? atof(e) : 0.2f;
   const dim3 grid(a->runs * a->Hk);
   auto run = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(*a); };
   if (a->D == 128) fp8 ? run(shared_prefix_kernel<128, true>)
                        : run(shared_prefix_kernel<128, false>);
   else fp8 ? run(shared_prefix_kernel<64, true>) : run(shared_prefix_kernel<64, false>);
-  const dim3 heads((a->Hq + 3) / 4, a->B);
+  const char* e3 = getenv("SP_MIX");
+  const bool wide = e3 && atoi(e3) < 2 ? atoi(e3) : a->B * a->Hq <= 1024;
+  const dim3 heads(wide ? a->Hq : (a->Hq + 3) / 4, a->B);
   auto join = [&](auto kernel) { kernel<<<heads, 256, 0, stream>>>(*a); };
-  a->D == 128 ? join(shared_prefix_join_kernel<128>) : join(shared_prefix_join_kernel<64>);
+  if (a->D == 128) wide ? join(shared_prefix_join_kernel<128, 4>)
+                        : join(shared_prefix_join_kernel<128, 1>);
+  else wide ? join(shared_prefix_join_kernel<64, 4>)
+            : join(shared_prefix_join_kernel<64, 1>);
 }
