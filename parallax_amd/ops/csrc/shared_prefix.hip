@@ -35,7 +35,8 @@
 #include "decode_tiles.h"
 
 #define SP_KT 64       // keys of a prefix tile
-#define SP_ITEMS 128   // items of one
+#define SP_ITEMS 128   // items of one: 4 waves x 32
+#define SP_THREADS 256
 #define SP_UNIT 32     // tokens of a suffix tile
 #define SP_GROUPS 256  // at most
 #define SP_ROWS 4096   // at most
@@ -98,6 +99,18 @@ DEVINL int page_at(const SharedPrefix& a, int entry) {
   return min(max(entry, 0), a.num_pages - 1);
 }
 
+// log2(e) cap tanh(x) of x = y / cap, y2 = 2 log2(e) x: off by some 2^-22 of the cap,
+// also where x is small, and that is what a weight's error goes by
+DEVINL float capped(float y2, float cap) {
+  const float e = __builtin_amdgcn_exp2f(y2);
+  return cap * kLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e));
+}
+
+// n / g of n below 2^20, exactly: n + 1/2 is 1/32 at least from where a quotient changes
+DEVINL int over(int n, int g) {
+  return (int)(((float)n + 0.5f) * __builtin_amdgcn_rcpf((float)g));
+}
+
 template <class F>
 DEVINL float over_halves(float v, F f) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v),
@@ -134,8 +147,8 @@ template <int D, bool FP8>
 DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const int hk,
                         const int run, const int total, const int runs) {
   constexpr int KCH = D / 8;            // 16-byte chunks of a K row
-  constexpr int KPER = SP_KT * KCH / 256;  // chunks that a thread copies
-  constexpr int VPER = D * 8 / 256;
+  constexpr int KPER = SP_KT * KCH / SP_THREADS;  // chunks that a thread copies
+  constexpr int VPER = D * 8 / SP_THREADS;
   constexpr int KSTEPS = D / 16;
   constexpr int DT = D / 32;
   const int tid = threadIdx.x;
@@ -177,32 +190,31 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   }
 
   // ---- what a lane copies and reads -------------------------------------------------
-  // 16 chunks (256 bytes) make a turn over the banks: a K row of 128 values, or two of
-  // 64; a V row has 64 tokens, so two as well
-  auto k_swz = [](int r) INL { return D == 128 ? r & 15 : (r >> 1) & 7; };
-  auto k_row = [&](int i) INL { return ((wid * KPER + i) * 64 + lane) / KCH; };
-  auto v_row = [&](int i) INL { return (wid * VPER + i) * 8 + (lane >> 3); };
-  auto v_src = [&](int i) INL { return (lane & 7) ^ ((v_row(i) >> 1) & 7); };
-  const uint32_t page_elems = (uint32_t)a.Hk * BS * D;
-  int koff[KPER], voff[VPER];
-#pragma unroll
-  for (int i = 0; i < KPER; ++i)
-    koff[i] = (hk * BS + (k_row(i) & (BS - 1))) * D + ((lane % KCH) ^ k_swz(k_row(i))) * 8;
-#pragma unroll
-  for (int i = 0; i < VPER; ++i)
-    voff[i] = (hk * D + v_row(i)) * BS + ((v_src(i) * 8) & (BS - 1));
+  // A wave copies 16 tokens, which lie in one page: of K two steps of 16 values at once,
+  // of V 32 rows. LDS holds both as operands are read, K as [16 tokens][step][token][16
+  // values], V as [16 tokens][row][16 tokens], the two chunks of 32 bytes exchanged
+  // every 8 rows: the lanes that read together then meet in no bank.
+  constexpr int ES = FP8 ? 1 : 2;
+  constexpr int GROUP = 16 * D;  // values of 16 tokens
+  const int line = (lane >> 1) & 15, chunk = (lane & 1) ^ ((lane >> 4) & 1);
+  const uint32_t page_bytes = (uint32_t)a.Hk * BS * D * ES;
+  const uint32_t in_page = (wid * 16) & (BS - 1);
+  const uint32_t koff =
+      ((hk * BS + in_page + line) * D + (lane >> 5) * 16 + chunk * 8) * ES;
+  const uint32_t voff = ((hk * D + (lane >> 1)) * BS + in_page + chunk * 8) * ES;
+  // K rows in the order that swaps bits 2 and 3
   const int krow = (l31 & 0x13) | ((l31 & 4) << 1) | ((l31 & 8) >> 1);
+  const int k_at = (krow >> 4) * GROUP + (krow & 15) * 16 + (half ^ ((krow >> 3) & 1)) * 8;
+  const int v_at = l31 * 16 + (half ^ ((l31 >> 3) & 1)) * 8;
   auto k_frag = [&](const uint16_t* Kl, int ks, int t) INL {
-    const int pos = (2 * ks + half) ^ k_swz(krow);
-    return *reinterpret_cast<const bf16x8v*>(Kl + (t * 32 + krow) * D + pos * 8);
+    return *reinterpret_cast<const bf16x8v*>(Kl + k_at + t * 2 * GROUP + ks * 256);
   };
   auto v_frag = [&](const uint16_t* Vl, int ks, int t) INL {
-    const int d = t * 32 + l31;
-    const int pos = (2 * ks + half) ^ ((d >> 1) & 7);
-    return *reinterpret_cast<const bf16x8v*>(Vl + d * SP_KT + pos * 8);
+    return *reinterpret_cast<const bf16x8v*>(Vl + v_at + ks * GROUP + t * 512);
   };
   // above 0 also for a scale of 0: hidden scores are multiplied by it too
   const float c = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1e-20f);
+  const float cap2 = 2.f * kLog2e * fabsf(a.scale) / fmaxf(a.softcap, 1e-30f);
 
   int done = 0;
   while (todo > 0) {
@@ -212,12 +224,12 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     const int kend = uniform(w.keys(g, &kb));
     kb = uniform(kb);
     const int keys = kend - kb;
-    const int tile = at / keys;
-    const int k0 = kb + at % keys, k1 = min(kend, k0 + todo);
+    const int tile = at < keys ? 0 : uniform(at / keys);
+    const int k0 = kb + at - tile * keys, k1 = min(kend, k0 + todo);
 
     // ---- the tile's items ---------------------------------------------------------
-    const int r0 = tile * SP_ITEMS / G;
-    const int r1 = (min((tile + 1) * SP_ITEMS, n_items) - 1) / G;
+    const int r0 = uniform(over(tile * SP_ITEMS, G));
+    const int r1 = uniform(over(min((tile + 1) * SP_ITEMS, n_items) - 1, G));
     __syncthreads();  // the buffers and the list are free
     if (wid == 0) {
       int rank = 0;
@@ -233,7 +245,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     __syncthreads();
     const int item = tile * SP_ITEMS + wid * 32 + l31;
     const bool on = item < n_items;
-    const int r = min(item, n_items - 1) / G;
+    const int r = over(min(item, n_items - 1), G);
     const int row = w.rows[r - r0];
     const int h = hk * G + min(item, n_items - 1) - r * G;
     const int lo = a.window > 0 ? window_start(a, a.lens[row]) : 0;
@@ -260,54 +272,49 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       const uint16_t* src = a.q + row * a.q_stride + h * D + half * 8;
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
-        u32x4v x = *reinterpret_cast<const u32x4v*>(src + s * 16);
-        if (a.scale < 0.f) x ^= 0x80008000u;  // the sign goes with q
-        qf[s] = __builtin_bit_cast(bf16x8v, x);
+        qf[s] = *reinterpret_cast<const bf16x8v*>(src + s * 16);
       }
     }
 
-    // Pages of the rows and chunks that this thread copies next: K's of tile kt, V's of
-    // tile vt. Tokens past the end are hidden later; their place is in the last page.
-    int kpage = 0, vpage[2] = {0, 0};
-    const int* vtable = (const int*)table;
-    auto pages = [&](int kt, int vt) INL {
-      kpage = page_at(a, table[min(kt * SP_KT + wid * 16, P - 1) >> a.shift]);
-      vpage[0] = page_at(a, vtable[min(vt * SP_KT + v_src(0) * 8, P - 1) >> a.shift]);
-      vpage[1] = page_at(a, vtable[min(vt * SP_KT + v_src(1) * 8, P - 1) >> a.shift]);
+    // Pages of the 16 tokens that this wave copies next, of K and of V, by the scalar
+    // unit a turn before. Tokens past the end are hidden later; their place is in the
+    // last page.
+    int kpage, vpage;
+    auto look = [&](int kt) INL {
+      return page_at(a, table[min(min(kt, k1 - 1) * SP_KT + wid * 16, P - 1) >> a.shift]);
     };
-    auto k_elem = [&](int i) INL {
-      return (uint64_t)(uint32_t)kpage * page_elems + (uint32_t)koff[i];
+    auto k_src = [&](int i) INL {
+      return a.k + (uint64_t)(uint32_t)kpage * page_bytes + i * 32 * ES + koff;
     };
-    auto v_elem = [&](int i) INL {
-      return (uint64_t)(uint32_t)vpage[i & 1] * page_elems + (uint32_t)voff[i];
+    auto v_src = [&](int i) INL {
+      return a.v + ((uint64_t)(uint32_t)vpage * page_bytes + (uint32_t)(i * 32 * BS * ES)) +
+             voff;
     };
-    auto copy_k = [&](uint16_t* Kl, int i) INL {
-      copy16_to_lds((const uint16_t*)a.k + k_elem(i), Kl + (wid * KPER + i) * 512);
-    };
-    auto copy_v = [&](uint16_t* Vl, int i) INL {
-      copy16_to_lds((const uint16_t*)a.v + v_elem(i), Vl + (wid * VPER + i) * 512);
-    };
+    // where a lane's chunk i goes: a copy writes 1 KB, 16 bytes a lane
+    auto to = [&](uint16_t* l, int i) INL { return l + wid * GROUP + i * 512; };
+    auto copy_k = [&](uint16_t* l, int i) INL { copy16_to_lds(k_src(i), to(l, i)); };
+    auto copy_v = [&](uint16_t* l, int i) INL { copy16_to_lds(v_src(i), to(l, i)); };
     uint64_t kraw[FP8 ? KPER : 1], vraw[FP8 ? VPER : 1];  // fp8 passes registers
     auto fetch_k = [&]() INL {
 #pragma unroll
       for (int i = 0; i < KPER; ++i)
-        kraw[i] = *reinterpret_cast<const uint64_t*>(a.k + k_elem(i));
+        kraw[i] = *reinterpret_cast<const uint64_t*>(k_src(i));
     };
     auto fetch_v = [&]() INL {
 #pragma unroll
       for (int i = 0; i < VPER; ++i)
-        vraw[i] = *reinterpret_cast<const uint64_t*>(a.v + v_elem(i));
+        vraw[i] = *reinterpret_cast<const uint64_t*>(v_src(i));
     };
-    auto settle_k = [&](uint16_t* Kl) INL {
+    auto settle_k = [&](uint16_t* l) INL {
 #pragma unroll
       for (int i = 0; i < KPER; ++i)
-        *reinterpret_cast<bf16x8v*>(Kl + ((wid * KPER + i) * 64 + lane) * 8) =
+        *reinterpret_cast<bf16x8v*>(to(l, i) + lane * 8) =
             widen((uint32_t)kraw[i], (uint32_t)(kraw[i] >> 32));
     };
-    auto settle_v = [&](uint16_t* Vl) INL {
+    auto settle_v = [&](uint16_t* l) INL {
 #pragma unroll
       for (int i = 0; i < VPER; ++i)
-        *reinterpret_cast<bf16x8v*>(Vl + ((wid * VPER + i) * 64 + lane) * 8) =
+        *reinterpret_cast<bf16x8v*>(to(l, i) + lane * 8) =
             widen((uint32_t)vraw[i], (uint32_t)(vraw[i] >> 32));
     };
 
@@ -356,16 +363,15 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     using none = std::integral_constant<int, 0>;
 
     // A turn takes the scores of tile kt and the weights and values of the tile before,
-    // which depend on nothing of this turn. Any turn: also the first and the last, a
-    // softcap, a mask.
+    // which depend on nothing of this turn. It copies K of the next tile and V of its
+    // own. Any turn: also the first and the last, a softcap, a mask.
     auto cut_turn = [&](int kt, const uint16_t* Kl, uint16_t* Kn, const uint16_t* Vl,
                         uint16_t* Vn) INL {
       const bool more = kt < k1, first = kt == k0;
       if (first) meet(std::integral_constant<int, FP8 ? 0 : KPER + VPER>{});
       else meet(none{});
-      if (more) {  // past the last tile K's copy is the last again
-        if (first) {
-        } else if constexpr (FP8) {
+      if (more && !first) {  // past the last tile K's copy is the last again
+        if constexpr (FP8) {
           fetch_k();
           fetch_v();
         } else {
@@ -374,53 +380,67 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
 #pragma unroll
           for (int i = 0; i < VPER; ++i) copy_v(Vn, i);
         }
-        pages(min(kt + 2, k1 - 1), min(kt + 1, k1 - 1));
+        vpage = kpage;
+        kpage = look(kt + 2);
       }
+      // operands are read AHEAD products early here too
+      constexpr int AHEAD = 4;
+      bf16x8v fr[AHEAD];
       if (wave_on && kt > k0) {
         const int base = (kt - 1) * SP_KT;
         const bool cut = base + SP_KT > P || base < lo_least;
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) fr[n] = v_frag(Vl, n / DT, n % DT);
         raise();
+        u32x4v w, keep;
 #pragma unroll
-        for (int ks = 0; ks < SP_KT / 16; ++ks) {
-          u32x4v w;
+        for (int n = 0; n < 4 * DT; ++n) {
+          const int ks = n / DT, t = n % DT;
+          if (t == 0) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = weigh(s0, ks, j);
-          bf16x8v v[DT];
+            for (int j = 0; j < 4; ++j) w[j] = weigh(s0, ks, j);
+            if (cut) {  // what no item sees may be anything: weight 0 times it
+              const int end = P - base - 16 * ks - 8 * half;
+              const int first = lo_least - base - 16 * ks - 8 * half;
 #pragma unroll
-          for (int t = 0; t < DT; ++t) v[t] = v_frag(Vl, ks, t);
-          if (cut) {  // what no item sees may be anything: weight 0 times it
-            const int end = P - base - 16 * ks - 8 * half;
-            const int first = lo_least - base - 16 * ks - 8 * half;
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                v[t][j] = j < end && j >= first ? v[t][j] : (short)0;
+              for (int j = 0; j < 4; ++j)
+                keep[j] = (2 * j >= first && 2 * j < end ? 0xffffu : 0u) |
+                          (2 * j + 1 >= first && 2 * j + 1 < end ? 0xffff0000u : 0u);
+            } else {
+              keep = u32x4v{~0u, ~0u, ~0u, ~0u};
+            }
           }
-#pragma unroll
-          for (int t = 0; t < DT; ++t)
-            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                v[t], __builtin_bit_cast(bf16x8v, w), o[t], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8v,
+                                 __builtin_bit_cast(u32x4v, fr[n % AHEAD]) & keep),
+              __builtin_bit_cast(bf16x8v, w), o[t], 0, 0, 0);
+          if (n + AHEAD < 4 * DT)
+            fr[n % AHEAD] = v_frag(Vl, (n + AHEAD) / DT, (n + AHEAD) % DT);
         }
         l += lsum;
         lsum = 0.f;
       }
       if (wave_on && more) {
         const int base = kt * SP_KT;
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) fr[n] = k_frag(Kl, n / 2, n % 2);
         s0[0] = s0[1] = f32x16v{};
 #pragma unroll
-        for (int ks = 0; ks < KSTEPS; ++ks)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            s0[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(Kl, ks, t), qf[ks],
-                                                            s0[t], 0, 0, 0);
+        for (int n = 0; n < 2 * KSTEPS; ++n) {
+          __builtin_amdgcn_sched_barrier(0);
+          s0[n % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[n % AHEAD], qf[n / 2],
+                                                              s0[n % 2], 0, 0, 0);
+          if (n + AHEAD < 2 * KSTEPS)
+            fr[n % AHEAD] = k_frag(Kl, (n + AHEAD) / 2, (n + AHEAD) % 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         if (a.softcap > 0.f) {
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              s0[t][e] =
-                  a.softcap * tanhf(s0[t][e] * fabsf(a.scale) / a.softcap) * kLog2e;
+              s0[t][e] = capped(s0[t][e] * cap2, a.softcap);
         }
         if (base + SP_KT > P || base < lo_most) {
           int end = P - base - 8 * half, first = lo - base - 8 * half;
@@ -462,7 +482,6 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       if constexpr (FP8) {
         fetch_k();
         fetch_v();
-        pages(min(kt + 2, k1 - 1), min(kt + 1, k1 - 1));
       }
 #pragma unroll
       for (int n = 0; n < NM; ++n) {
@@ -484,7 +503,10 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
         if constexpr (!FP8) {
           if (n < KPER) copy_k(Kn, n);
           else if (n - KPER < VPER) copy_v(Vn, n - KPER);
-          else if (n == KPER + VPER) pages(min(kt + 2, k1 - 1), min(kt + 1, k1 - 1));
+        }
+        if (n == KPER + VPER) {
+          vpage = kpage;
+          kpage = look(kt + 2);
         }
         if (n == NS) mx = larger(sn[0][0], sn[0]);
       }
@@ -504,26 +526,34 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
 
     // The first turn's K, and behind it what that turn would ask for: the buffers are
     // free, and short prefixes are rows of such waits.
-    pages(k0, k0);
-    const int second = page_at(a, table[min(min(k0 + 1, k1 - 1) * SP_KT + wid * 16, P - 1) >>
-                                        a.shift]);
-    if constexpr (FP8) {
-      fetch_k();
-      fetch_v();
-      settle_k(K0);
-      kpage = second;
-      fetch_k();
-      settle_v(V0);
-    } else {
+    {
+      kpage = vpage = look(k0);
+      const int second = look(k0 + 1), third = look(k0 + 2);
+      if constexpr (FP8) {
+        fetch_k();
+        fetch_v();
+        settle_k(K0);
+        kpage = second;
+        fetch_k();
+        settle_v(V0);
+      } else {
 #pragma unroll
-      for (int i = 0; i < KPER; ++i) copy_k(K0, i);
-      asm volatile("" ::: "memory");
-      kpage = second;
+        for (int i = 0; i < KPER; ++i) copy_k(K0, i);
+        asm volatile("" ::: "memory");
+        kpage = second;
 #pragma unroll
-      for (int i = 0; i < KPER; ++i) copy_k(K1, i);
+        for (int i = 0; i < KPER; ++i) copy_k(K1, i);
 #pragma unroll
-      for (int i = 0; i < VPER; ++i) copy_v(V0, i);
+        for (int i = 0; i < VPER; ++i) copy_v(V0, i);
+      }
+      vpage = second;
+      kpage = third;
     }
+    if (a.scale < 0.f)  // the sign goes with q; here, as it waits for q
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s)
+        qf[s] = __builtin_bit_cast(
+            bf16x8v, __builtin_bit_cast(u32x4v, qf[s]) ^ 0x80008000u);
     for (int kt = k0; kt <= k1; kt += 2) {
       for (; kt >= whole && kt + 1 < cut; kt += 2) {
         whole_turn(kt, K0, K1, V1, V0, s1, s0);
@@ -577,7 +607,8 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   constexpr int NC = TILE / 1024;        // copies of K, and of V
   constexpr int KC = D / 32;
   constexpr int MT = D / 16;
-  static_assert(4 * 2 * TILE <= tiles_bytes(D) && SP_ROWS * 4 <= tiles_bytes(D), "");
+  constexpr int W = SP_THREADS / 64;
+  static_assert(W * 2 * TILE <= tiles_bytes(D) && SP_ROWS * 4 <= tiles_bytes(D), "");
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wid = uniform(tid >> 6);
@@ -586,8 +617,8 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   const int G = a.Hq / a.Hk, BS = 1 << a.shift;
 
   // ---- this wave's run of tiles --------------------------------------------------------
-  const int wave = run * 4 + wid;
-  const int per = max((total + 4 * runs - 1) / (4 * runs), 1);
+  const int wave = run * W + wid;
+  const int per = max((total + W * runs - 1) / (W * runs), 1);
   const int begin = wave * per;
   const int todo = uniform(max(0, min(per, total - begin)));
   int seq = 0, at = 0, before = 0;
@@ -624,6 +655,7 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       FP8 ? lds_at(Vt) + l15 * VB + ((l4 >> 1) ^ swz_v<FP8>(l15)) * 16 + (l4 & 1) * 8
           : lds_at(Vt) + l15 * VB + (l4 ^ swz_v<FP8>(l15)) * 16;
   const float c = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1e-20f);
+  const float cap2 = 2.f * kLog2e * fabsf(a.scale) / fmaxf(a.softcap, 1e-30f);
 
   // Rows 64 at a time, one a lane: where its own tokens begin and end.
   int rows0 = -64, row_lo = 0, row_end = 0;
@@ -762,9 +794,7 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     if (a.softcap > 0.f) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        s[e >> 2][e & 3] = a.softcap *
-                           tanhf(s[e >> 2][e & 3] * fabsf(a.scale) / a.softcap) *
-                           kLog2e;
+        s[e >> 2][e & 3] = capped(s[e >> 2][e & 3] * cap2, a.softcap);
     }
     const bool cut = tok + KT > L || tok < lo;
     if (cut) {
@@ -865,7 +895,7 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
 }  // namespace
 
 template <int D, bool FP8>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(
+__global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_kernel(
     const SharedPrefix a) {
   __shared__ __attribute__((aligned(1024))) uint8_t S[lds_bytes(D)];
   const int hk = blockIdx.x % a.Hk, run = blockIdx.x / a.Hk;
@@ -878,7 +908,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(
   w.rows = w.low + SP_GROUPS;
   w.member = (int16_t*)(w.rows + SP_ITEMS + 4);
   int* const sum = w.rows;  // of all units
-  for (int g = tid; g < a.N; g += 256) {
+  int L = 0, group = -1;  // of this thread's first row, asked for with the prefixes
+  if (tid < a.B) {
+    L = a.lens[tid];
+    group = a.group[tid];
+  }
+  for (int g = tid; g < a.N; g += SP_THREADS) {
     w.prefix[g] = a.prefix[g];
     w.count[g] = 0;
     w.low[g] = INT_MAX;
@@ -886,8 +921,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(
   if (tid == 0) *sum = 0;
   __syncthreads();
   int mine = 0;
-  for (int b = tid; b < a.B; b += 256) {
-    const int L = a.lens[b], g = a.group[b];
+  for (int b = tid; b < a.B; b += SP_THREADS) {
+    if (b >= SP_THREADS) {
+      L = a.lens[b];
+      group = a.group[b];
+    }
+    const int g = group;
     int P = g >= 0 && g < a.N ? w.prefix[g] : 0;
     if (P <= 0 || L < P) P = 0;
     const int lo = window_start(a, L);
@@ -915,6 +954,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void shared_prefix_kernel(
   __syncthreads();  // the sum is read
   const float p_cost = p_total, s_cost = s_total * a.ratio;
   int p_runs = (int)(a.runs * (p_cost / (p_cost + s_cost)) + 0.5f);
+  p_runs = uniform(p_runs);
   p_runs = p_total == 0 ? 0 : s_total == 0 ? a.runs : min(max(p_runs, 1), a.runs - 1);
   if (run < p_runs)
     prefix_role<D, FP8>(a, w, S, hk, run, p_total, p_runs);
@@ -1019,7 +1059,7 @@ extern "C" void launch_shared_prefix(const SharedPrefix* a_, bool fp8, hipStream
   const char* e = getenv("SP_S");
   a2.ratio = e ? atof(e) : 0.2f;
   const dim3 grid(a->runs * a->Hk);
-  auto run = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(*a); };
+  auto run = [&](auto kernel) { kernel<<<grid, SP_THREADS, 0, stream>>>(*a); };
   if (a->D == 128) fp8 ? run(shared_prefix_kernel<128, true>)
                        : run(shared_prefix_kernel<128, false>);
   else fp8 ? run(shared_prefix_kernel<64, true>) : run(shared_prefix_kernel<64, false>);
