@@ -55,7 +55,7 @@ struct SharedPrefix {
   int window;
   int runs;      // workgroups of a key/value head
   float ratio;
-  float* p_acc;  // [p_parts, Hk, SP_ITEMS, D]: part run + item tile
+  float* p_acc;  // [p_parts, Hk, SP_ITEMS, D]: part run, or run + item tile
   float* p_ml;   // [p_parts, Hk, SP_ITEMS, 2] maxima in units of log2, sums
   int4* p_info;  // [B, Hq]: first part, parts, place in them; rows of a group only
   float* s_acc;  // [s_parts, Hq, D]: part wave + row
@@ -158,23 +158,46 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   const int l31 = lane & 31;
   const int G = a.Hq / a.Hk, BS = 1 << a.shift;
 
-  uint16_t* const K0 = (uint16_t*)S;
-  uint16_t* const V0 = K0 + SP_KT * D;
-  uint16_t* const K1 = V0 + SP_KT * D;
-  uint16_t* const V1 = K1 + SP_KT * D;
+  constexpr int TILE = SP_KT * D;
+  uint16_t* const K0 = (uint16_t*)S;  // K and V of two tiles
+  uint16_t* const V0 = K0 + TILE;
+  uint16_t* const K1 = V0 + TILE;
+  uint16_t* const V1 = K1 + TILE;
 
   // ---- this workgroup's run of key tiles ------------------------------------------
-  const int per = max((total + runs - 1) / runs, 1);
-  const int begin = run * per;
-  if (begin >= total) return;
-  int todo = min(per, total - begin);
-  int g = 0, at = 0, tile0 = 0, before = 0;
+  // Where there are no more item tiles than workgroups, each has a run of one item
+  // tile's key tiles, the shortest length that this gives for all; otherwise equal runs
+  // of the list of all of them. A run's begin and end cost as much as four key tiles.
+  auto sum_over_groups = [&](auto f) INL {  // of f(group), for groups with rows
+    int all = 0;
+    for (int g0 = 0; g0 < a.N; g0 += 64) {
+      const int x = g0 + lane;
+      all += of_lane(sum_to_lane(x < a.N && w.count[x] > 0 ? f(x) : 0), 63);
+    }
+    return all;
+  };
+  auto keys_of = [&](int x) INL {
+    int kb;
+    const int end = w.keys(x, &kb);
+    return end - kb;
+  };
+  int per = uniform(max((total + runs - 1) / runs, 1));
+  const bool apart = sum_over_groups([&](int x) { return w.tiles(x, G); }) <= runs;
+  while (apart) {  // ends where per is the longest group's at the latest
+    const int n = sum_over_groups(
+        [&](int x) { return w.tiles(x, G) * ((keys_of(x) + per - 1) / per); });
+    if (n <= runs) break;
+    per = uniform(max(per + 1, (int)((float)per * n / runs)));
+  }
+  // the group that has this run: its place in the list of what is dealt
+  const int begin = apart ? run : run * per;
+  int g = 0, at = -1, tile0 = 0, before = 0;
   for (int g0 = 0; g0 < a.N; g0 += 64) {
     const int x = g0 + lane;
-    int kb, n = 0, t = 0;
+    int n = 0, t = 0;
     if (x < a.N && w.count[x] > 0) {
       t = w.tiles(x, G);
-      n = t * (w.keys(x, &kb) - kb);
+      n = t * (apart ? (keys_of(x) + per - 1) / per : keys_of(x));
     }
     const int ns = sum_to_lane(n), ts = sum_to_lane(t);
     const unsigned long long hit = __ballot(before + ns > begin);
@@ -187,6 +210,16 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     }
     before += of_lane(ns, 63);
     tile0 += of_lane(ts, 63);
+  }
+  if (at < 0) return;  // nothing is left for it
+  int todo = uniform(min(per, total - begin));
+  if (apart) {
+    const int keys = uniform(keys_of(g)), n = uniform((keys + per - 1) / per);
+    const int tile = uniform(at / n), i = at - tile * n;
+    per = uniform((keys + n - 1) / n);  // even
+    at = tile * keys + i * per;
+    todo = min(per, keys - i * per);
+    if (todo <= 0) return;
   }
 
   // ---- what a lane copies and reads -------------------------------------------------
@@ -261,10 +294,12 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     }
     lo_most = uniform(lo_most);
     const int lo_least = uniform(w.low[g]);
+    const int part0 = apart ? run : run + tile0 + tile;
 
     if (k0 == kb && half == 0 && on)
       a.p_info[(int64_t)row * a.Hq + h] =
-          make_int4(run + tile0 + tile, (begin + done + keys - 1) / per - run + 1,
+          make_int4(part0, apart ? (keys + per - 1) / per
+                                 : (begin + done + keys - 1) / per - run + 1,
                     item - tile * SP_ITEMS, 0);
 
     bf16x8v qf[KSTEPS];
@@ -362,11 +397,36 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     };
     using none = std::integral_constant<int, 0>;
 
+    // What no item sees of a tile's V may be anything, also no number, and its weight 0
+    // times it: zeros in its place. Only where a mask cuts the tile for all.
+    auto clean = [&](int base, uint16_t* Vl) INL {
+      const int end = P - base - wid * 16, first = lo_least - base - wid * 16;
+      u32x4v keep[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = 8 * (i ^ ((lane >> 3) & 1)) + 2 * j;
+          keep[i][j] = (tok >= first && tok < end ? 0xffffu : 0u) |
+                       (tok + 1 >= first && tok + 1 < end ? 0xffff0000u : 0u);
+        }
+#pragma unroll 1
+      for (int d = lane; d < D; d += 64) {  // rows that leave the lane's bit 3 as it is
+        u32x4v* row = reinterpret_cast<u32x4v*>(Vl + wid * GROUP + d * 16);
+        row[0] &= keep[0];
+        row[1] &= keep[1];
+      }
+    };
+
     // A turn takes the scores of tile kt and the weights and values of the tile before,
     // which depend on nothing of this turn. It copies K of the next tile and V of its
-    // own. Any turn: also the first and the last, a softcap, a mask.
-    auto cut_turn = [&](int kt, const uint16_t* Kl, uint16_t* Kn, const uint16_t* Vl,
-                        uint16_t* Vn) INL {
+    // own. Any turn: also the first and the last, a softcap, a mask. `odd` (0 or 1): of
+    // a segment's turns, which begin with K0 and V0.
+    auto cut_turn = [&](int kt, int odd) INL {
+      const uint16_t* Kl = K0 + odd * (2 * TILE);
+      uint16_t* Kn = K1 - odd * (2 * TILE);
+      uint16_t* Vl = V1 - odd * (2 * TILE);
+      uint16_t* Vn = V0 + odd * (2 * TILE);
       const bool more = kt < k1, first = kt == k0;
       if (first) meet(std::integral_constant<int, FP8 ? 0 : KPER + VPER>{});
       else meet(none{});
@@ -383,38 +443,27 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
         vpage = kpage;
         kpage = look(kt + 2);
       }
+      if (!first && (kt * SP_KT > P || (kt - 1) * SP_KT < lo_least)) {
+        clean((kt - 1) * SP_KT, Vl);
+        __syncthreads();
+      }
       // operands are read AHEAD products early here too
       constexpr int AHEAD = 4;
       bf16x8v fr[AHEAD];
-      if (wave_on && kt > k0) {
-        const int base = (kt - 1) * SP_KT;
-        const bool cut = base + SP_KT > P || base < lo_least;
+      if (wave_on && !first) {
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) fr[n] = v_frag(Vl, n / DT, n % DT);
         raise();
-        u32x4v w, keep;
+        u32x4v w;
 #pragma unroll
         for (int n = 0; n < 4 * DT; ++n) {
           const int ks = n / DT, t = n % DT;
-          if (t == 0) {
+          if (t == 0)
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = weigh(s0, ks, j);
-            if (cut) {  // what no item sees may be anything: weight 0 times it
-              const int end = P - base - 16 * ks - 8 * half;
-              const int first = lo_least - base - 16 * ks - 8 * half;
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                keep[j] = (2 * j >= first && 2 * j < end ? 0xffffu : 0u) |
-                          (2 * j + 1 >= first && 2 * j + 1 < end ? 0xffff0000u : 0u);
-            } else {
-              keep = u32x4v{~0u, ~0u, ~0u, ~0u};
-            }
-          }
           __builtin_amdgcn_sched_barrier(0);
           o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8v,
-                                 __builtin_bit_cast(u32x4v, fr[n % AHEAD]) & keep),
-              __builtin_bit_cast(bf16x8v, w), o[t], 0, 0, 0);
+              fr[n % AHEAD], __builtin_bit_cast(bf16x8v, w), o[t], 0, 0, 0);
           if (n + AHEAD < 4 * DT)
             fr[n % AHEAD] = v_frag(Vl, (n + AHEAD) / DT, (n + AHEAD) % DT);
         }
@@ -443,15 +492,15 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
               s0[t][e] = capped(s0[t][e] * cap2, a.softcap);
         }
         if (base + SP_KT > P || base < lo_most) {
-          int end = P - base - 8 * half, first = lo - base - 8 * half;
-          asm volatile("" : "+v"(end));  // not computed where no mask is applied
-          asm volatile("" : "+v"(first));
+          int begin = lo - base - 8 * half;  // tokens [begin, begin + count) are seen
+          uint32_t count = max(P - lo, 0);
+          asm volatile("" : "+v"(begin));  // not computed where no mask is applied
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const int tok = 32 * t + 16 * (e >> 3) + (e & 7);
-              s0[t][e] = tok < end && tok >= first ? s0[t][e] : kHidden;
+              s0[t][e] = (uint32_t)(tok - begin) < count ? s0[t][e] : kHidden;
             }
         }
         mx = top_of(larger(larger(s0[0][0], s0[0]), s0[1]));
@@ -554,18 +603,18 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       for (int s = 0; s < KSTEPS; ++s)
         qf[s] = __builtin_bit_cast(
             bf16x8v, __builtin_bit_cast(u32x4v, qf[s]) ^ 0x80008000u);
-    for (int kt = k0; kt <= k1; kt += 2) {
-      for (; kt >= whole && kt + 1 < cut; kt += 2) {
-        whole_turn(kt, K0, K1, V1, V0, s1, s0);
-        whole_turn(kt + 1, K1, K0, V0, V1, s0, s1);
-      }
-      cut_turn(kt, K0, K1, V1, V0);
-      if (kt + 1 <= k1) cut_turn(kt + 1, K1, K0, V0, V1);
+    for (int kt = k0, odd = 0; kt <= k1; ++kt, odd ^= 1) {
+      if (odd == 0)
+        for (; kt >= whole && kt + 1 < cut; kt += 2) {
+          whole_turn(kt, K0, K1, V1, V0, s1, s0);
+          whole_turn(kt + 1, K1, K0, V0, V1, s0, s1);
+        }
+      cut_turn(kt, odd);
     }
 
     l = over_halves(l, [](float x, float y) { return x + y; });
     if (on) {
-      const int64_t part = ((int64_t)(run + tile0 + tile) * a.Hk + hk) * SP_ITEMS +
+      const int64_t part = ((int64_t)part0 * a.Hk + hk) * SP_ITEMS +
                            item - tile * SP_ITEMS;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
@@ -582,6 +631,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     todo -= k1 - k0;
     done += k1 - k0;
     at += k1 - k0;
+    if (apart) break;
     const int tiles = uniform(w.tiles(g, G));
     if (at == tiles * keys) {
       at = 0;
