@@ -18,37 +18,7 @@
 #include <optional>
 #include <utility>
 
-struct HeadNormStore {
-  uint16_t* out;
-  const uint16_t *q, *k, *v, *q_w, *k_w;
-  void *k_cache, *v_cache;
-  const int* positions;
-  const float* cos_sin;
-  const int64_t* slots;
-  int T, Hq, Hk, D, rot, BS, P;
-  int64_t num_slots;
-  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
-  float eps, inv_k, inv_v;
-};
-
-struct SharedPrefix {
-  uint16_t* out;
-  const uint16_t* q;
-  const uint8_t *k, *v;
-  const int *tables, *lens, *group, *prefix;
-  const float* sinks;
-  int B, N, Hq, Hk, D, shift, max_blocks, num_pages;
-  int64_t q_stride;
-  float scale, v_scale, softcap;
-  int window;
-  int runs;
-  float ratio;
-  float *p_acc, *p_ml;
-  int4* p_info;
-  float *s_acc, *s_ml;
-  int2* s_info;
-  int* has;
-};
+#include "cache_ops.h"
 
 extern "C" {
 void launch_head_norm_store(const HeadNormStore*, bool, bool, hipStream_t);

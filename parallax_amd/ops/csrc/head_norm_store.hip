@@ -12,6 +12,7 @@
 // A position outside the table makes NaN and a slot outside the cache stores nothing:
 // both are the caller's fault, and neither may read or write past a buffer.
 
+#include "cache_ops.h"
 #include "common.h"
 
 namespace {
@@ -27,19 +28,6 @@ DEVINL uint8_t to_e4m3(float x) {
 }
 
 }  // namespace
-
-struct HeadNormStore {
-  uint16_t* out;  // [T, Hq, D]
-  const uint16_t *q, *k, *v, *q_w, *k_w;
-  void *k_cache, *v_cache;  // [NB, Hk, BS, D], [NB, Hk, D, BS]
-  const int* positions;
-  const float* cos_sin;  // [P, rot]
-  const int64_t* slots;
-  int T, Hq, Hk, D, rot, BS, P;
-  int64_t num_slots;
-  int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides
-  float eps, inv_k, inv_v;
-};
 
 // Any sizes: a wave a head, whose normed values lie in LDS for the pairs.
 template <bool NEOX, bool FP8>

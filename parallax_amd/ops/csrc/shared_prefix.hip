@@ -27,9 +27,9 @@
 
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 #include <type_traits>
 
+#include "cache_ops.h"
 #include "common.h"
 #include "decode_common.h"
 #include "decode_tiles.h"
@@ -42,27 +42,6 @@
 #define SP_ROWS 4096   // at most
 
 typedef float f32x16v __attribute__((ext_vector_type(16)));
-
-struct SharedPrefix {
-  uint16_t* out;           // [B, Hq, D]
-  const uint16_t* q;       // [B, Hq, D] rows at q_stride
-  const uint8_t *k, *v;    // [NB, Hk, BS, D], [NB, Hk, D, BS], bf16 | fp8
-  const int *tables, *lens, *group, *prefix;  // [B, max_blocks], [B], [B], [N]
-  const float* sinks;      // [Hq] or null
-  int B, N, Hq, Hk, D, shift, max_blocks, num_pages;
-  int64_t q_stride;
-  float scale, v_scale, softcap;  // scale: with that of an fp8 cache's keys
-  int window;
-  int runs;      // workgroups of a key/value head
-  float ratio;
-  float* p_acc;  // [p_parts, Hk, SP_ITEMS, D]: part run, or run + item tile
-  float* p_ml;   // [p_parts, Hk, SP_ITEMS, 2] maxima in units of log2, sums
-  int4* p_info;  // [B, Hq]: first part, parts, place in them; rows of a group only
-  float* s_acc;  // [s_parts, Hq, D]: part wave + row
-  float* s_ml;   // [s_parts, Hq, 2]
-  int2* s_info;  // [B]: first and last wave; rows with tokens behind a prefix only
-  int* has;      // [B]: 1: of a prefix, + 2: behind one
-};
 
 namespace {
 
@@ -181,7 +160,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     const int end = w.keys(x, &kb);
     return end - kb;
   };
-  int per = uniform(max((total + runs - 1) / runs, 1));
+  int per = uniform(max((total + runs - 1) / runs, total >= 64 ? 2 : 1));
   const bool apart = sum_over_groups([&](int x) { return w.tiles(x, G); }) <= runs;
   while (apart) {  // ends where per is the longest group's at the latest
     const int n = sum_over_groups(
@@ -604,7 +583,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
         qf[s] = __builtin_bit_cast(
             bf16x8v, __builtin_bit_cast(u32x4v, qf[s]) ^ 0x80008000u);
     for (int kt = k0, odd = 0; kt <= k1; ++kt, odd ^= 1) {
-      if (odd == 0)
+      if (D == 128 && odd == 0)
         for (; kt >= whole && kt + 1 < cut; kt += 2) {
           whole_turn(kt, K0, K1, V1, V0, s1, s0);
           whole_turn(kt + 1, K1, K0, V0, V1, s0, s1);
@@ -668,7 +647,7 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
 
   // ---- this wave's run of tiles --------------------------------------------------------
   const int wave = run * W + wid;
-  const int per = max((total + W * runs - 1) / (W * runs), 1);
+  const int per = max((total + 4 * runs - 1) / (4 * runs), 1);
   const int begin = wave * per;
   const int todo = uniform(max(0, min(per, total - begin)));
   int seq = 0, at = 0, before = 0;
@@ -1002,7 +981,7 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
     p_total += of_lane(sum_to_lane(n), 63);
   }
   __syncthreads();  // the sum is read
-  const float p_cost = p_total, s_cost = s_total * a.ratio;
+  const float p_cost = p_total, s_cost = s_total * 0.25f;
   int p_runs = (int)(a.runs * (p_cost / (p_cost + s_cost)) + 0.5f);
   p_runs = uniform(p_runs);
   p_runs = p_total == 0 ? 0 : s_total == 0 ? a.runs : min(max(p_runs, 1), a.runs - 1);
@@ -1094,27 +1073,22 @@ __global__ __launch_bounds__(256) void shared_prefix_join_kernel(const SharedPre
         make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
 }
 
-// Workgroups of a key/value head, and the item tiles that B rows of N groups make at
-// most.
+// Workgroups of a key/value head, as many as the chip holds at once, and the item tiles
+// that B rows of N groups make at most.
 extern "C" void shared_prefix_plan(int B, int N, int Hq, int Hk, int D, int* runs,
                                    int* tiles) {
-  const char* e = getenv("SP_P");
-  *runs = std::max(2, (e && atoi(e) ? atoi(e) : D == 128 ? 512 : 768) / Hk);
+  *runs = std::max(2, (D == 128 ? 512 : 768) / Hk);
   *tiles = N > 0 ? (int)((int64_t)B * (Hq / Hk) / SP_ITEMS) + std::min(N, B) : 0;
 }
 
-extern "C" void launch_shared_prefix(const SharedPrefix* a_, bool fp8, hipStream_t stream) {
-  SharedPrefix a2 = *a_;
-  SharedPrefix* a = &a2;
-  const char* e = getenv("SP_S");
-  a2.ratio = e ? atof(e) : 0.2f;
+extern "C" void launch_shared_prefix(const SharedPrefix* a, bool fp8, hipStream_t stream) {
   const dim3 grid(a->runs * a->Hk);
   auto run = [&](auto kernel) { kernel<<<grid, SP_THREADS, 0, stream>>>(*a); };
   if (a->D == 128) fp8 ? run(shared_prefix_kernel<128, true>)
                        : run(shared_prefix_kernel<128, false>);
   else fp8 ? run(shared_prefix_kernel<64, true>) : run(shared_prefix_kernel<64, false>);
-  const char* e3 = getenv("SP_MIX");
-  const bool wide = e3 && atoi(e3) < 2 ? atoi(e3) : a->B * a->Hq <= 1024;
+  // few rows: four waves each, which share its parts
+  const bool wide = a->B * a->Hq <= 1024;
   const dim3 heads(wide ? a->Hq : (a->Hq + 3) / 4, a->B);
   auto join = [&](auto kernel) { kernel<<<heads, 256, 0, stream>>>(*a); };
   if (a->D == 128) wide ? join(shared_prefix_join_kernel<128, 4>)
