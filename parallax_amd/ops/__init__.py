@@ -157,8 +157,10 @@ def qk_norm_rope_and_cache(
     A slot below 0 or past the cache stores nothing (rows that pad a batch); a position
     outside the table makes NaN; two rows of one slot leave either's values. There is no
     gradient: inputs that require one are refused."""
-    positions = positions.to(torch.int32)
-    slot_mapping = slot_mapping.to(torch.int64)
+    if positions.dtype is not torch.int32:
+        positions = positions.to(torch.int32)
+    if slot_mapping.dtype is not torch.int64:
+        slot_mapping = slot_mapping.to(torch.int64)
     if q.is_cuda:
         return _require_ext("qk_norm_rope_and_cache").qk_norm_rope_and_cache(
             q, k, v, q_weight, k_weight, eps, k_cache, v_cache, positions, cos_sin,
@@ -307,7 +309,8 @@ def shared_prefix_attention_decode(
     At most 4096 rows, 256 groups and 16 query heads a key/value head of 64 or 128.
     There is no gradient: a q that requires one is refused."""
     block_tables, seq_lens, prefix_group, prefix_lens = (
-        t.to(torch.int32) for t in (block_tables, seq_lens, prefix_group, prefix_lens))
+        t if t.dtype is torch.int32 else t.to(torch.int32)
+        for t in (block_tables, seq_lens, prefix_group, prefix_lens))
     if sinks is not None:
         sinks = sinks.float()
     if q.is_cuda:

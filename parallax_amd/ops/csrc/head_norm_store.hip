@@ -11,6 +11,11 @@
 //
 // A position outside the table makes NaN and a slot outside the cache stores nothing:
 // both are the caller's fault, and neither may read or write past a buffer.
+//
+// What bounds it: prompts memory, 8,192 tokens of 32 and 8 heads of 128 in bf16 (206 MB)
+// 38.5 us or 5.3 TB/s in a row of calls, 42 among calls on other tensors; into an fp8
+// cache 36. Decode latency: one token 2.7 us, 96 4.1, 200 rows of 64 and 8 heads
+// into an fp8 cache 6.1. Copies, norms and rope_and_cache() apart: one token 6.9.
 
 #include <type_traits>
 
@@ -325,6 +330,10 @@ extern "C" void launch_head_norm_store(const HeadNormStore* a, bool neox, bool f
              : run(head_norm_store_kernel<false, false>);
     return;
   }
+  // Runs of slots and two heads a lane for prompts, a token's eight values a thread for
+  // decode. us without / with, 32 and 8 heads of 128 in bf16, two prompts: 256 tokens 5.6
+  // / 5.5, 512 8.4 / 5.6, 2,048 21 / 11.2, 8,192 84 / 38.5 (one head a lane 40.4, four
+  // 39.8); 96 and 256 requests of a slot each 4.1 / 12.3 and 6.9 / 14.8.
   const bool many = a->T >= 512;
   const int64_t eights = (int64_t)a->Hk * (a->D / 8);
   const int64_t v_blocks =
@@ -345,7 +354,7 @@ extern "C" void launch_head_norm_store(const HeadNormStore* a, bool neox, bool f
     else fp8 ? run(lph, u, no, yes, runs) : run(lph, u, no, no, runs);
   };
   auto width = [&](auto lph) {
-    if (many) flags(lph, std::integral_constant<int, 4>{}, std::true_type{});
+    if (many) flags(lph, std::integral_constant<int, 2>{}, std::true_type{});
     else flags(lph, std::integral_constant<int, 1>{}, std::false_type{});
   };
   if (a->D <= 64) width(std::integral_constant<int, 4>{});
