@@ -306,8 +306,17 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     };
     // where a lane's chunk i goes: a copy writes 1 KB, 16 bytes a lane
     auto to = [&](uint16_t* l, int i) INL { return l + wid * GROUP + i * 512; };
-    auto copy_k = [&](uint16_t* l, int i) INL { copy16_to_lds(k_src(i), to(l, i)); };
-    auto copy_v = [&](uint16_t* l, int i) INL { copy16_to_lds(v_src(i), to(l, i)); };
+    auto copy = [&](const uint8_t* page, uint32_t off, uint32_t more, uint16_t* l) INL {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          __builtin_amdgcn_make_buffer_rsrc((void*)page, 0, (int)page_bytes, 0x00027000),
+          (__attribute__((address_space(3))) void*)l, 16, off, more, 0, 0);
+    };
+    auto copy_k = [&](uint16_t* l, int i) INL {
+      copy(a.k + (uint64_t)(uint32_t)kpage * page_bytes, koff, i * 32 * ES, to(l, i));
+    };
+    auto copy_v = [&](uint16_t* l, int i) INL {
+      copy(a.v + (uint64_t)(uint32_t)vpage * page_bytes, voff, i * 32 * BS * ES, to(l, i));
+    };
     uint64_t kraw[FP8 ? KPER : 1], vraw[FP8 ? VPER : 1];  // fp8 passes registers
     auto fetch_k = [&]() INL {
 #pragma unroll
