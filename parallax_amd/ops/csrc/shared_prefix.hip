@@ -40,6 +40,7 @@
 #define SP_UNIT 32     // tokens of a suffix tile
 #define SP_GROUPS 256  // at most
 #define SP_ROWS 4096   // at most
+#define SP_SPANS 512
 
 typedef float f32x16v __attribute__((ext_vector_type(16)));
 
@@ -99,7 +100,7 @@ DEVINL float over_halves(float v, F f) {
 
 constexpr int tiles_bytes(int D) { return 4 * SP_KT * D * 2; }
 constexpr int lds_bytes(int D) {
-  return tiles_bytes(D) + (3 * SP_GROUPS + SP_ITEMS + 4) * 4 + SP_ROWS * 2;
+  return tiles_bytes(D) + (3 * SP_GROUPS + SP_ITEMS + 4) * 4 + SP_SPANS * 8 + SP_ROWS * 2;
 }
 
 // What a workgroup finds of the batch, in LDS behind its tiles.
@@ -108,6 +109,7 @@ struct Lists {
   int* count;       // rows of a group
   int* low;         // where the first window of a group's rows begins
   int* rows;        // of an item tile; [SP_ITEMS]: its group's first row
+  int2* span;       // of the first SP_SPANS rows: where a row's own tokens begin and end
   int16_t* member;  // a row's group, -1: none
   int* units;       // a row's suffix tiles; here the tiles come to lie
 
@@ -118,13 +120,28 @@ struct Lists {
     *begin = min(low[g] / SP_KT, end - 1);
     return end;
   }
+  DEVINL int key_tiles(int g) const {
+    int begin;
+    const int end = keys(g, &begin);
+    return end - begin;
+  }
+  template <class F>
+  DEVINL int sum_over(int groups, F f) const {  // of f(group), for groups with rows
+    const int lane = threadIdx.x & 63;
+    int all = 0;
+    for (int g0 = 0; g0 < groups; g0 += 64) {
+      const int g = g0 + lane;
+      all += of_lane(sum_to_lane(g < groups && count[g] > 0 ? f(g) : 0), 63);
+    }
+    return all;
+  }
 };
 
 // ---- prefixes ----------------------------------------------------------------------
 
 template <int D, bool FP8>
 DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const int hk,
-                        const int run, const int total, const int runs) {
+                        const int run, const int total, int per, const bool apart) {
   constexpr int KCH = D / 8;            // 16-byte chunks of a K row
   constexpr int KPER = SP_KT * KCH / SP_THREADS;  // chunks that a thread copies
   constexpr int VPER = D * 8 / SP_THREADS;
@@ -144,30 +161,6 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   uint16_t* const V1 = K1 + TILE;
 
   // ---- this workgroup's run of key tiles ------------------------------------------
-  // Where there are no more item tiles than workgroups, each has a run of one item
-  // tile's key tiles, the shortest length that this gives for all; otherwise equal runs
-  // of the list of all of them. A run's begin and end cost as much as four key tiles.
-  auto sum_over_groups = [&](auto f) INL {  // of f(group), for groups with rows
-    int all = 0;
-    for (int g0 = 0; g0 < a.N; g0 += 64) {
-      const int x = g0 + lane;
-      all += of_lane(sum_to_lane(x < a.N && w.count[x] > 0 ? f(x) : 0), 63);
-    }
-    return all;
-  };
-  auto keys_of = [&](int x) INL {
-    int kb;
-    const int end = w.keys(x, &kb);
-    return end - kb;
-  };
-  int per = uniform(max((total + runs - 1) / runs, total >= 64 ? 2 : 1));
-  const bool apart = sum_over_groups([&](int x) { return w.tiles(x, G); }) <= runs;
-  while (apart) {  // ends where per is the longest group's at the latest
-    const int n = sum_over_groups(
-        [&](int x) { return w.tiles(x, G) * ((keys_of(x) + per - 1) / per); });
-    if (n <= runs) break;
-    per = uniform(max(per + 1, (int)((float)per * n / runs)));
-  }
   // the group that has this run: its place in the list of what is dealt
   const int begin = apart ? run : run * per;
   int g = 0, at = -1, tile0 = 0, before = 0;
@@ -176,7 +169,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     int n = 0, t = 0;
     if (x < a.N && w.count[x] > 0) {
       t = w.tiles(x, G);
-      n = t * (apart ? (keys_of(x) + per - 1) / per : keys_of(x));
+      n = t * (apart ? (w.key_tiles(x) + per - 1) / per : w.key_tiles(x));
     }
     const int ns = sum_to_lane(n), ts = sum_to_lane(t);
     const unsigned long long hit = __ballot(before + ns > begin);
@@ -193,7 +186,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   if (at < 0) return;  // nothing is left for it
   int todo = uniform(min(per, total - begin));
   if (apart) {
-    const int keys = uniform(keys_of(g)), n = uniform((keys + per - 1) / per);
+    const int keys = uniform(w.key_tiles(g)), n = uniform((keys + per - 1) / per);
     const int tile = uniform(at / n), i = at - tile * n;
     per = uniform((keys + n - 1) / n);  // even
     at = tile * keys + i * per;
@@ -700,13 +693,16 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   unsigned long long filled = 0, grouped = 0;
   auto look = [&](int b0) INL {
     rows0 = b0;
-    const int b = min(b0 + lane, a.B - 1);
-    const int g = a.group[b];
-    row_end = a.lens[b];
-    int P = g >= 0 && g < a.N ? w.prefix[g] : 0;
-    if (P <= 0 || row_end < P) P = 0;
-    row_lo = max(P, window_start(a, row_end));
-    grouped = __ballot(P > 0);
+    const int b = min(b0 + lane, a.B - 1), g = w.member[b];
+    if (b0 < SP_SPANS) {
+      const int2 x = w.span[min(b, SP_SPANS - 1)];
+      row_lo = x.x;
+      row_end = x.y;
+    } else {
+      row_end = a.lens[b];
+      row_lo = max(g >= 0 ? w.prefix[g] : 0, window_start(a, row_end));
+    }
+    grouped = __ballot(g >= 0);
     filled = __ballot(b0 + lane < a.B && row_lo < row_end);
   };
   // One tile after the other, across rows: while one is computed, the next is copied
@@ -944,7 +940,8 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
   w.count = w.prefix + SP_GROUPS;
   w.low = w.count + SP_GROUPS;
   w.rows = w.low + SP_GROUPS;
-  w.member = (int16_t*)(w.rows + SP_ITEMS + 4);
+  w.span = (int2*)(w.rows + SP_ITEMS + 4);
+  w.member = (int16_t*)(w.span + SP_SPANS);
   int* const sum = w.rows;  // of all units
   int L = 0, group = -1;  // of this thread's first row, asked for with the prefixes
   if (tid < a.B) {
@@ -974,6 +971,7 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
       atomicMin(w.low + g, lo);
     }
     const int n = suffix_units(max(P, lo), L);
+    if (b < SP_SPANS) w.span[b] = make_int2(max(P, lo), L);
     w.units[b] = n;
     mine += n;
     if (blockIdx.x == 0) a.has[b] = (P > 0) + 2 * (n > 0);
@@ -982,20 +980,39 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
   if (lane == 63) atomicAdd(sum, mine);
   __syncthreads();
   const int s_total = uniform(*sum);
-  int p_total = 0;
-  for (int g0 = 0; g0 < a.N; g0 += 64) {
-    const int g = g0 + lane;
-    int kb, n = 0;
-    if (g < a.N && w.count[g] > 0) n = w.tiles(g, a.Hq / a.Hk) * (w.keys(g, &kb) - kb);
-    p_total += of_lane(sum_to_lane(n), 63);
-  }
+  const int G = a.Hq / a.Hk;
+  const int tiles = w.sum_over(a.N, [&](int g) { return w.tiles(g, G); });
+  const int p_total =
+      w.sum_over(a.N, [&](int g) { return w.tiles(g, G) * w.key_tiles(g); });
   __syncthreads();  // the sum is read
-  const float p_cost = p_total, s_cost = s_total * 0.25f;
-  int p_runs = (int)(a.runs * (p_cost / (p_cost + s_cost)) + 0.5f);
-  p_runs = uniform(p_runs);
-  p_runs = p_total == 0 ? 0 : s_total == 0 ? a.runs : min(max(p_runs, 1), a.runs - 1);
+
+  // Workgroups for prefixes, by what the key tiles and the suffix tiles cost.
+  int p_runs = 0, per = 1;
+  bool apart = false;
+  if (p_total > 0) {
+    p_runs = a.runs;
+    if (s_total > 0) {
+      const float p_cost = p_total, s_cost = s_total * (FP8 ? 0.25f : 0.3f);
+      p_runs = uniform((int)(a.runs * (p_cost / (p_cost + s_cost)) + 0.5f));
+      p_runs = min(max(p_runs, 1), a.runs - 1);
+    }
+    // Where there are no more item tiles than workgroups, each has a run of one item
+    // tile's key tiles, the shortest length that this gives for all; otherwise equal runs
+    // of the list of all of them. A run's begin and end cost as much as four key tiles.
+    per = uniform(max((p_total + p_runs - 1) / p_runs, p_total >= 64 ? 2 : 1));
+    apart = tiles <= p_runs;
+    int used = (p_total + per - 1) / per;
+    while (apart) {  // ends where per is the longest group's at the latest
+      used = w.sum_over(a.N, [&](int g) {
+        return w.tiles(g, G) * ((w.key_tiles(g) + per - 1) / per);
+      });
+      if (used <= p_runs) break;
+      per = uniform(max(per + 1, (int)((float)per * used / p_runs)));
+    }
+    p_runs = uniform(used);  // the others are for suffixes
+  }
   if (run < p_runs)
-    prefix_role<D, FP8>(a, w, S, hk, run, p_total, p_runs);
+    prefix_role<D, FP8>(a, w, S, hk, run, p_total, per, apart);
   else
     suffix_role<D, FP8>(a, w, S, hk, run - p_runs, s_total, a.runs - p_runs);
 }
@@ -1004,7 +1021,7 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
 // the weights; groups of D / 4 lanes take the parts in turn, in a fixed order.
 template <int D, int W>
 __global__ __launch_bounds__(256) void shared_prefix_join_kernel(const SharedPrefix a) {
-  constexpr int Q = D / 4, GROUPS = 64 / Q, AHEAD = 4;
+  constexpr int Q = D / 4, GROUPS = 64 / Q, AHEAD = W > 1 ? 4 : 2;
   __shared__ f32x4v sums[W > 1 ? W : 1][Q];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int h = W > 1 ? blockIdx.x : blockIdx.x * 4 + wid, b = blockIdx.y;
