@@ -869,28 +869,32 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     read_rows(vr, v_at);
     issue_v(t1);
     const Tile t2 = i + 2 < todo ? next(t1) : t1;
+    bf16x8v vb[MT];
+#pragma unroll
+    for (int d = 0; d < MT; ++d) {
+      if constexpr (FP8)
+        vb[d] = widen(vr[d][0], vr[d][1]);
+      else
+        vb[d] = __builtin_bit_cast(bf16x8v, vr[d]);
+    }
     // slots past the end, and before the row's own tokens, may hold anything:
     // weight 0 times it
-    u32x4v keep = {~0u, ~0u, ~0u, ~0u};
     if (cut) {
       const int first = lo - tok - 8 * l4, end = L - tok - 8 * l4;
+      u32x4v keep;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         keep[j] = (2 * j >= first && 2 * j < end ? 0xffffu : 0u) |
                   (2 * j + 1 >= first && 2 * j + 1 < end ? 0xffff0000u : 0u);
+      asm volatile("" : "+v"(keep));  // a branch, not 32 instructions for every tile
+#pragma unroll
+      for (int d = 0; d < MT; ++d)
+        vb[d] = __builtin_bit_cast(bf16x8v, __builtin_bit_cast(u32x4v, vb[d]) & keep);
     }
     const bf16x8v pb = __builtin_bit_cast(bf16x8v, pk);
 #pragma unroll
-    for (int d = 0; d < MT; ++d) {
-      u32x4v x;
-      if constexpr (FP8)
-        x = __builtin_bit_cast(u32x4v, widen(vr[d][0], vr[d][1]));
-      else
-        x = vr[d];
-      if (cut) x &= keep;
-      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-          __builtin_bit_cast(bf16x8v, x), pb, o[d], 0, 0, 0);
-    }
+    for (int d = 0; d < MT; ++d)
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb[d], pb, o[d], 0, 0, 0);
 
     // ---- out: column l15 = head, rows of O^T = d -----------------------------------------
     if (t1.row != t0.row || i + 1 == todo) {
