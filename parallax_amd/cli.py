@@ -194,6 +194,12 @@ def add_engine_args(p: argparse.ArgumentParser) -> None:
     p.add_argument("--decode-priority", action="store_true",
                    help="form decode batches before prefills (lower TPOT "
                         "under arrival bursts at the cost of TTFT)")
+    p.add_argument("--fused-head-norms", action="store_true",
+                   help="models with norms of heads: norms, rotation and cache append "
+                        "in one launch")
+    p.add_argument("--shared-prefix-attention", action="store_true",
+                   help="decode batches read the pages of a prefix that their requests "
+                        "share once (system prompts, one document asked about often)")
     p.add_argument("--tp-size", type=int, default=1,
                    help="tensor-parallel degree; ranks = tp x pp "
                         "(torchrun --nproc-per-node must equal tp*pp)")
@@ -242,6 +248,8 @@ def engine_args_from_cli(args, world: int = 1):
         prefill_priority=not args.decode_priority,
         moe_weight_dtype=args.moe_weight_dtype,
         linear_weight_dtype=args.linear_weight_dtype,
+        fused_head_norms=args.fused_head_norms,
+        shared_prefix_attention=args.shared_prefix_attention,
     )
 
 

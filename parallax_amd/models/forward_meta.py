@@ -46,6 +46,10 @@ class ForwardMeta:
     # and slot_mapping that token's place (below 0 for rows that pad the batch), so
     # that a layer may store it and attend in one launch
     appends: bool = False
+    # decode only: the group of rows that share a prefix, -1 for none, and the tokens
+    # that each group shares (server/shared_prefix.py); not together with `appends`
+    prefix_group: Optional[torch.Tensor] = None  # [B] int32
+    prefix_lens: Optional[torch.Tensor] = None   # [groups] int32
     # derived per-token tables for packed-sequence kernels (built on first
     # use, shared by every layer of the forward)
     _token_seq: Optional[torch.Tensor] = None

@@ -125,6 +125,10 @@ class ResidualLayerNorm(nn.Module):
 
 
 class LlamaAttention(nn.Module):
+    # norms of heads, rotation and append in one launch, the normed heads not rounded in
+    # between (EngineArgs.fused_head_norms sets it on a module)
+    fused_head_norms = False
+
     def __init__(self, cfg: ModelConfig, layer_idx: int, local_layer_idx: int):
         super().__init__()
         comm = get_comm()
@@ -179,7 +183,14 @@ class LlamaAttention(nn.Module):
         q = q.view(T, self.num_heads, self.head_dim)
         k = k.view(T, self.num_kv_heads, self.head_dim)
         v = v.view(T, self.num_kv_heads, self.head_dim)
-        if self.qk_norm:
+        k_cache, v_cache = meta.kv_cache.layer(self.local_layer_idx)
+        sinks = self.sinks.float() if self.sinks is not None else None
+        fused = self.fused_head_norms and self.qk_norm and not self.qk_norm_full
+        if fused:
+            q = ops.qk_norm_rope_and_cache(
+                q, k, v, self.q_norm.weight, self.k_norm.weight, self.q_norm.eps,
+                k_cache, v_cache, meta.positions, rope_cache, meta.slot_mapping)
+        elif self.qk_norm:
             if self.qk_norm_full:
                 q = self.q_norm(q.reshape(T, -1)).view(T, self.num_heads, self.head_dim)
                 k = self.k_norm(k.reshape(T, -1)).view(T, self.num_kv_heads, self.head_dim)
@@ -187,9 +198,7 @@ class LlamaAttention(nn.Module):
                 q = self.q_norm(q.contiguous())
                 k = self.k_norm(k.contiguous())
             v = v.contiguous()
-        k_cache, v_cache = meta.kv_cache.layer(self.local_layer_idx)
-        sinks = self.sinks.float() if self.sinks is not None else None
-        if meta.appends:
+        if meta.appends and not fused:
             attn = ops.rope_cache_attention_decode(
                 q, k, v, k_cache, v_cache, meta.positions, rope_cache,
                 meta.slot_mapping, meta.block_tables, meta.seq_lens, self.scale,
@@ -198,15 +207,22 @@ class LlamaAttention(nn.Module):
             if attn is not None:
                 return self._project_out(attn, x, T) if project else attn.reshape(
                     T, self.num_heads * self.head_dim)
-        ops.rope_and_cache(
-            q, k, v, k_cache, v_cache, meta.positions, rope_cache,
-            meta.slot_mapping,
-        )
+        if not fused:
+            ops.rope_and_cache(
+                q, k, v, k_cache, v_cache, meta.positions, rope_cache,
+                meta.slot_mapping,
+            )
 
         if meta.is_prefill:
             attn = ops.prefill_attention(
                 q, k_cache, v_cache, meta.block_tables, meta.seq_lens,
                 meta.query_lens, self.scale, self.sliding_window, sinks=sinks,
+            )
+        elif meta.prefix_group is not None:
+            attn = ops.shared_prefix_attention_decode(
+                q, k_cache, v_cache, meta.block_tables, meta.seq_lens,
+                meta.prefix_group, meta.prefix_lens, self.scale, self.sliding_window,
+                sinks=sinks,
             )
         else:
             attn = ops.paged_attention_decode(

@@ -27,6 +27,7 @@ from .. import ops
 from ..models import get_model_class
 from ..models.config import ModelConfig
 from ..models.forward_meta import ForwardMeta
+from ..models.llama import LlamaAttention
 from ..parallel.comm import CommContext, get_comm
 from ..utils.logging_config import get_logger
 from .cache_manager import CacheManager
@@ -41,6 +42,7 @@ from .request import InitialRequest, new_request_id
 from .sampler import Sampler
 from .sampling_params import SamplingParams
 from .scheduler import PrefillChunk, Scheduler
+from .shared_prefix import SharedPrefixes
 
 logger = get_logger("server.engine")
 
@@ -82,6 +84,12 @@ class EngineArgs:
     # recurrent-state slots kept beyond max_batch_size (requests that finish
     # one step late under async decode still hold theirs)
     extra_linear_slots: int = 8
+    # norms of heads, rotation and append in one launch; the normed heads are not rounded
+    # in between, so results are not bit for bit those of the default
+    fused_head_norms: bool = False
+    # decode batches whose prompts begin alike read the pages of their shared prefixes
+    # once, where that saves enough (server/shared_prefix.py)
+    shared_prefix_attention: bool = False
 
 
 def partition_layers(num_layers: int, pp_size: int, pp_rank: int) -> Tuple[int, int]:
@@ -269,6 +277,12 @@ class Engine:
             prefill_priority=args.prefill_priority,
         )
         self.sampler = Sampler(self.device, args.seed)
+        if args.fused_head_norms:
+            self._fuse_head_norms()
+        self.shared_prefixes = None
+        if args.shared_prefix_attention:
+            self._check_shared_prefixes()
+            self.shared_prefixes = SharedPrefixes(self.kv_cache.spec)
         self.graph_runner = None
         if args.enable_graphs and self.device.type == "cuda" \
                 and getattr(self.model, "graph_safe", True):
@@ -283,6 +297,7 @@ class Engine:
                 is_mla=self.is_mla,
                 linear_cache=self.linear_cache,
                 linear_scratch_slot=args.max_batch_size + args.extra_linear_slots,
+                shared_prefixes=self.shared_prefixes,
             )
         self._pending_adds: List[InitialRequest] = []
         self._inflight = None       # async decode pipelining state
@@ -303,6 +318,39 @@ class Engine:
             start, end, cfg.num_layers, num_blocks, args.block_size,
             self.is_mla, self.device,
         )
+
+    def _attentions(self) -> List[LlamaAttention]:
+        """The attention modules whose steps are LlamaAttention's own."""
+        return [m for m in self.model.modules() if isinstance(m, LlamaAttention)
+                and type(m).forward is LlamaAttention.forward
+                and type(m).attend is LlamaAttention.attend]
+
+    def _fuse_head_norms(self) -> None:
+        modules = [m for m in self._attentions() if m.qk_norm and not m.qk_norm_full]
+        if not modules:
+            raise ValueError(
+                f"fused_head_norms: {self.cfg.architecture} has no norms of single heads")
+        if self.device.type == "cuda" and self.args.dtype != torch.bfloat16:
+            raise ValueError("fused_head_norms needs bfloat16")
+        for m in modules:
+            m.fused_head_norms = True
+
+    def _check_shared_prefixes(self) -> None:
+        modules = self._attentions()
+        if not modules or self.is_mla or self.cfg.has_linear_layers or len(modules) < sum(
+                isinstance(m, LlamaAttention) for m in self.model.modules()):
+            raise ValueError(f"shared_prefix_attention: {self.cfg.architecture} has "
+                             "layers without it")
+        if not self.args.enable_prefix_cache:
+            raise ValueError("shared_prefix_attention needs the prefix cache")
+        if self.device.type == "cuda" and (
+                self.args.dtype != torch.bfloat16
+                or self.args.block_size not in (16, 32, 64)
+                or any(m.head_dim not in (64, 128)
+                       or m.num_heads > 16 * m.num_kv_heads for m in modules)):
+            raise ValueError(
+                "shared_prefix_attention needs bfloat16, pages of 16, 32 or 64 tokens, "
+                "heads of 64 or 128 and at most 16 query heads a key/value head")
 
     # -- public API (head rank) ----------------------------------------------------
 
@@ -838,12 +886,18 @@ class Engine:
             block_tables.append(state.block_table)
             seq_lens.append(pos + 1)
         dev = self.device
+        shared = self.shared_prefixes and self.shared_prefixes.find(block_tables,
+                                                                    seq_lens)
+        group, lens = [torch.tensor(x, dtype=torch.int32, device=dev) for x in shared] \
+            if shared else (None, None)
         meta = ForwardMeta(
             is_prefill=False,
             positions=torch.tensor(positions, dtype=torch.int32, device=dev),
             slot_mapping=torch.tensor(slot_mapping, dtype=torch.int64, device=dev),
             block_tables=build_block_table_tensor(block_tables, dev),
             seq_lens=torch.tensor(seq_lens, dtype=torch.int32, device=dev),
+            prefix_group=group,
+            prefix_lens=lens,
             kv_cache=None if self.is_mla else self.kv_cache,
             mla_cache=self.kv_cache if self.is_mla else None,
             linear_cache=self.linear_cache,
@@ -856,7 +910,7 @@ class Engine:
             prev_ids=torch.tensor([r.decode_prev() for r in reqs],
                                   dtype=torch.long, device=dev)
             if self.uses_prev_tokens else None,
-            appends=True,
+            appends=not shared,
         )
         ids = torch.tensor(input_ids, dtype=torch.long, device=dev)
         return meta, ids

@@ -22,6 +22,8 @@ Capture-shape invariants:
   max_model_len): short contexts replay a graph whose attention grid has few
   flash-decoding partitions instead of carrying max_model_len's empty ones
   (~0.5 us per 1k empty workgroups per call adds up over 32-61 layers).
+- batches that share prefixes (server/shared_prefix.py) replay a graph of their own per
+  batch bucket: its attention deals the work on the device, whatever the contexts.
 """
 
 from __future__ import annotations
@@ -33,8 +35,11 @@ import torch
 
 from ..models.forward_meta import ForwardMeta
 from ..utils.logging_config import get_logger
+from .shared_prefix import MAX_GROUPS, MAX_ROWS
 
 logger = get_logger("server.graph_runner")
+
+SHARED = 0  # in place of a context bucket: the graph of batches that share prefixes
 
 DEFAULT_BUCKETS = [1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 160, 192, 224, 256,
                    384, 512, 768]
@@ -57,6 +62,7 @@ class DecodeGraphRunner:
         is_mla: bool = False,
         linear_cache=None,
         linear_scratch_slot: int = 0,
+        shared_prefixes=None,
     ):
         self.is_mla = is_mla
         # hybrid stacks (deltanet/lightning): per-request state slots; pad
@@ -113,6 +119,12 @@ class DecodeGraphRunner:
             self.h_linear_slots = torch.full((B,), linear_scratch_slot,
                                              dtype=torch.int64, pin_memory=True)
 
+        self.shared_prefixes = shared_prefixes
+        if shared_prefixes is not None:
+            # groups of the rows, -1 behind them, and what each group shares
+            self.prefix_group = torch.full((B,), -1, dtype=torch.int32, device=dev)
+            self.prefix_lens = torch.zeros(MAX_GROUPS, dtype=torch.int32, device=dev)
+
         self.ctx_buckets: List[int] = []
         c = 1024
         while c < max_model_len:
@@ -132,8 +144,10 @@ class DecodeGraphRunner:
         # its request ended names a new table (other pages), and holding the
         # old list keeps its identity from being recycled
         self._cached_tables: List[List[int]] = []
+        self._cached_shared = None
 
     def _meta(self, bucket: int, ctx_bucket: Optional[int] = None) -> ForwardMeta:
+        shared = ctx_bucket == SHARED
         return ForwardMeta(
             is_prefill=False,
             positions=self.positions[:bucket],
@@ -148,7 +162,9 @@ class DecodeGraphRunner:
             linear_slots=self.linear_slots[:bucket]
             if self.linear_cache is not None else None,
             prev_ids=self.prev_ids[:bucket] if self.uses_prev else None,
-            appends=True,
+            appends=not shared,
+            prefix_group=self.prefix_group[:bucket] if shared else None,
+            prefix_lens=self.prefix_lens if shared else None,
         )
 
     def _forward(self, bucket: int, ctx_bucket: Optional[int] = None) -> torch.Tensor:
@@ -177,6 +193,9 @@ class DecodeGraphRunner:
         self.slot_mapping.fill_(-1)
         self.block_tables.zero_()
         self.seq_lens.fill_(1)
+        if self.shared_prefixes is not None:
+            self.prefix_group.fill_(-1)
+            self.prefix_lens.zero_()
         if self.linear_cache is not None:
             self.linear_slots.fill_(self.linear_scratch_slot)
         torch.cuda.synchronize()
@@ -210,6 +229,9 @@ class DecodeGraphRunner:
             for c in self.ctx_buckets:
                 if (b, c) not in self._graphs:
                     self._capture(b, c)
+            if self.shared_prefixes is not None and 1 < b <= MAX_ROWS \
+                    and (b, SHARED) not in self._graphs:
+                self._capture(b, SHARED)
         logger.info("pre-captured %d decode graphs in %.1fs",
                     len(self._graphs), time.monotonic() - t0)
 
@@ -242,6 +264,10 @@ class DecodeGraphRunner:
         B = len(seq_lens)
         bucket = self.bucket_for(B)
         ctx_bucket = self.ctx_bucket_for(max(seq_lens))
+        shared = self.shared_prefixes and bucket <= MAX_ROWS \
+            and self.shared_prefixes.find(block_tables, seq_lens)
+        if shared:
+            ctx_bucket = SHARED
         key = (bucket, ctx_bucket)
         if key not in self._graphs:
             self._capture(bucket, ctx_bucket)
@@ -280,6 +306,13 @@ class DecodeGraphRunner:
         self._cached_rids = list(rids) if rids is not None else []
         self._cached_btlens = btlens
         self._cached_tables = list(block_tables)
+        if shared and not (same_batch and shared is self._cached_shared):
+            for dst, src, pad in ((self.prefix_group, shared[0], -1),
+                                  (self.prefix_lens, shared[1], 0)):
+                dst.copy_(torch.tensor(
+                    src + [pad] * (dst.shape[0] - len(src)), dtype=torch.int32,
+                    pin_memory=True), non_blocking=True)
+            self._cached_shared = shared
 
         if self.uses_prev:
             if input_ids_dev is None:
