@@ -218,7 +218,7 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   shared_prefix_plan(a.B, a.N, a.Hq, a.Hk, a.D, &a.runs, &tiles);
   // fp32 words: of a part its sums, then maxima and sums of weights; then where a row's
   // parts lie
-  const int64_t p_items = N > 0 ? (int64_t)(a.runs + tiles) * Hk * 256 : 0;
+  const int64_t p_items = N > 0 ? (int64_t)(a.runs + tiles) * Hk * 128 : 0;
   const int64_t s_items = (4 * a.runs + B) * Hq;
   const int64_t words = (p_items + s_items) * (D + 2) + B * Hq * 4 + B * 3;
   auto work = torch::empty({words}, q.options().dtype(at::kFloat));

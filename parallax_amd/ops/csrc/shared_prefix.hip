@@ -46,10 +46,9 @@ typedef float f32x16v __attribute__((ext_vector_type(16)));
 
 namespace {
 
-DEVINL int prefix_of(const SharedPrefix& a, int b) {
-  const int g = a.group[b];
-  const int p = g >= 0 && g < a.N ? a.prefix[g] : 0;
-  return p > 0 && a.lens[b] >= p ? p : 0;
+// tokens of a row, of those that its table has pages for
+DEVINL int length(const SharedPrefix& a, int b) {
+  return min(a.lens[b], a.max_blocks << a.shift);
 }
 
 DEVINL int window_start(const SharedPrefix& a, int L) {
@@ -253,7 +252,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     const int r = over(min(item, n_items - 1), G);
     const int row = w.rows[r - r0];
     const int h = hk * G + min(item, n_items - 1) - r * G;
-    const int lo = a.window > 0 ? window_start(a, a.lens[row]) : 0;
+    const int lo = a.window > 0 ? window_start(a, length(a, row)) : 0;
     // constant memory: read by the scalar unit
     const auto* table = (const __attribute__((address_space(4))) int*)(
         a.tables + (size_t)uniform(w.rows[SP_ITEMS]) * a.max_blocks);
@@ -699,7 +698,7 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       row_lo = x.x;
       row_end = x.y;
     } else {
-      row_end = a.lens[b];
+      row_end = length(a, b);
       row_lo = max(g >= 0 ? w.prefix[g] : 0, window_start(a, row_end));
     }
     grouped = __ballot(g >= 0);
@@ -949,7 +948,7 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
   int* const sum = w.rows;  // of all units
   int L = 0, group = -1;  // of this thread's first row, asked for with the prefixes
   if (tid < a.B) {
-    L = a.lens[tid];
+    L = length(a, tid);
     group = a.group[tid];
   }
   for (int g = tid; g < a.N; g += SP_THREADS) {
@@ -962,7 +961,7 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
   int mine = 0;
   for (int b = tid; b < a.B; b += SP_THREADS) {
     if (b >= SP_THREADS) {
-      L = a.lens[b];
+      L = length(a, b);
       group = a.group[b];
     }
     const int g = group;

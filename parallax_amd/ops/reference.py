@@ -257,7 +257,8 @@ def shared_prefix_attention_decode(
     Hk, block_size = k_cache.shape[1:3]
     out = torch.zeros_like(q)
     first = {}
-    lens, prefix = seq_lens.tolist(), prefix_lens.tolist()
+    lens = seq_lens.clamp(max=block_tables.shape[1] * block_size).tolist()
+    prefix = prefix_lens.tolist()
     for b, (L, g) in enumerate(zip(lens, prefix_group.tolist())):
         P = prefix[g] if 0 <= g < len(prefix) and 0 < prefix[g] <= L else 0
         if L <= 0:

@@ -32,6 +32,17 @@ def test_cpu_form_is_decode():
     assert (got.float() - want.float()).abs().max() < 0.02
 
 
+def test_lengths_past_the_table():
+    """A row that claims more tokens than its table has pages for ends with the table;
+    a prefix past that has no rows."""
+    s = prefix_inputs(4, 2, 64, 16, [(0, 48), (0, 48), (1, 48)], [20, 60])
+    s["tables"] = s["tables"][:, :3].contiguous()
+    want = prefix_oracle(s)
+    s["lens"] = torch.tensor([48, 49, 2 ** 31 - 1], dtype=torch.int32)
+    assert_attended(prefix_call(ops.shared_prefix_attention_decode, s, "cpu"), want,
+                    weights=0.0)
+
+
 def bad_calls():
     x, i = torch.randn, torch.int32
     b = torch.bfloat16

@@ -262,3 +262,85 @@ def test_steps_together():
         now = {**grown, "q": out.cpu().view(B, -1), "kc": kc.cpu(), "vc": vc.cpu(),
                "lens": lens}
         assert_attended(prefix_call(OP, now, "cuda"), prefix_oracle(now))
+
+
+def test_lengths_past_the_table():
+    s = prefix_inputs(4, 2, 64, 16, [(0, 48), (0, 48), (1, 48)], [20, 60])
+    s["tables"] = s["tables"][:, :3].contiguous()
+    want = prefix_oracle(s)
+    s["lens"] = torch.tensor([48, 49, 2 ** 31 - 1], dtype=torch.int32)
+    assert_attended(prefix_call(OP, s, "cuda"), want)
+
+
+@pytest.mark.parametrize("Hk,D,groups,prefix", [
+    (32, 64, 40, 150),    # 24 workgroups a head, 40 tiles of items
+    (64, 128, 20, 500),   # 8 and 20
+    (300, 64, 3, 70),     # 2 and 3
+    (400, 128, 1, 200),   # 2, of which one takes suffixes
+    (1, 64, 256, 130),    # all groups that there can be
+])
+def test_tiles_and_workgroups(Hk, D, groups, prefix):
+    """More tiles of items than workgroups: runs that go from one group to the next."""
+    r = random.Random(Hk)
+    lens = [prefix + r.randint(-60, 60) for _ in range(groups)]
+    rows = [(g, lens[g] + r.randint(0, 40)) for g in range(groups) for _ in range(3)]
+    r.shuffle(rows)
+    check(prefix_inputs(Hk, Hk, D, 16, rows, lens, seed=Hk))
+
+
+def test_only_prefixes():
+    """No row has a token of its own."""
+    check(prefix_inputs(8, 2, 128, 16, [(0, 700)] * 20 + [(1, 64)] * 3, [700, 64]))
+    check(prefix_inputs(64, 64, 128, 16, [(g, 100) for g in range(20)] * 2, [100] * 20))
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_any(seed):
+    """Rows, groups, heads, pages, windows as they come."""
+    r = random.Random(100 + seed)
+    Hk, D, BS = r.choice([1, 2, 3, 8]), r.choice([64, 128]), r.choice([16, 32, 64])
+    Hq = Hk * r.choice([1, 2, 5, 7, 8, 16])
+    prefix = [r.choice([0, 1, 17, 64, 100, 400, 1500]) for _ in range(r.randint(0, 12))]
+    rows = []
+    for _ in range(r.choice([1, 3, 17, 64, 150])):
+        g = r.randint(-1, len(prefix))
+        P = prefix[g] if 0 <= g < len(prefix) else 0
+        rows.append((g, max(0, r.choice([P, P, P, 0]) + r.choice([-1, 0, 1, 30, 200]))))
+    kw = {}
+    if r.random() < 0.4:
+        kw["sliding_window"] = r.choice([1, 30, 64, 200, 1000])
+    if r.random() < 0.3:
+        kw["softcap"] = r.choice([1.0, 20.0])
+    if r.random() < 0.3:
+        kw["sinks"] = torch.randn(Hq, generator=torch.Generator().manual_seed(seed)).cuda()
+    check(prefix_inputs(Hq, Hk, D, BS, rows, prefix, fp8=r.random() < 0.5, seed=seed,
+                        q_gap=r.choice([0, 8])), **kw)
+
+
+def test_two_at_once():
+    """Calls on two streams and graphs replayed on both, each with results of its own."""
+    a = prefix_inputs(8, 2, 64, 16, ODD, [200, 129])
+    b = prefix_inputs(16, 2, 128, 32, shared(30, 900, 100), [900], fp8=True)
+    want = [prefix_call(OP, s, "cuda") for s in (a, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    args, graphs, outs = [], [], []
+    for s in (a, b):
+        B, Hq, D = s["shape"]
+        args.append([s["q"].cuda().view(B, Hq, D)] + [s[n].cuda() for n in (
+            "kc", "vc", "tables", "lens", "group", "prefix")] + [D ** -0.5, -1, 0.0, None,
+                                                                 *s["scales"]])
+    torch.cuda.synchronize()
+    for x in args:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(OP(*x))
+        graphs.append(g)
+    for _ in range(20):
+        eager = []
+        for s, g, x in zip(streams, graphs, args):
+            with torch.cuda.stream(s):
+                g.replay()
+                eager.append(OP(*x))
+        torch.cuda.synchronize()
+        for w, o, e in zip(want, outs, eager):
+            assert torch.equal(o, w) and torch.equal(e, w)
