@@ -24,6 +24,21 @@
 //
 // Lengths, groups and prefixes are read on the device, by every workgroup itself; the
 // grid depends on sizes alone.
+//
+// What bounds it, replayed in graphs, 32 query heads over 8 of 128 in bf16 unless said:
+// Long prefixes by the products with the softmax's instructions beside them: 64 rows, 64
+// heads over 8, 60,000 shared tokens 154 us, 816 TFLOP/s, where a product of 8192^3 by
+// itself reaches 1,213; of an fp8 cache 151, 184 with up to 4,000 more tokens a row.
+// Suffixes by the stream of their keys and values: 8 rows over 100,000, where the prefix
+// is little more than a stream too, 90 us, 4.6 TB/s. Both together: 256 rows over 8,000,
+// up to 600 of their own, 98, of which the prefix alone is 57 and the rest alone 89. Small
+// batches by waits in a row, of lengths, lists, page numbers, a tile, and by the second
+// launch: 4 rows over 700 tokens, 14 heads over 2 of 64, 10.5; 16 rows over 500, up to 300
+// of their own, 14.9, where paged_decode.hip starts with 6. The second launch is 4 to 10
+// of each, 9 where it reads the 20 MB of 8,192 heads' parts.
+//
+// Keys and values of 16-bit caches go to LDS by buffer instructions: behind global ones
+// the compiler waits for all reads of LDS at once, 164 us where these took 151.
 
 #include <algorithm>
 #include <climits>
@@ -583,6 +598,9 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       for (int s = 0; s < KSTEPS; ++s)
         qf[s] = __builtin_bit_cast(
             bf16x8v, __builtin_bit_cast(u32x4v, qf[s]) ^ 0x80008000u);
+    // Whole turns apart only of 128: with heads of 64 the compiler runs out of the 168
+    // registers of three workgroups a CU; without / with, us: eight groups of 16 rows
+    // over 2,000 in bf16 37.8 / 39.3, 256 rows over 8,000 in fp8 70.5 / 69.0.
     for (int kt = k0, odd = 0; kt <= k1; ++kt, odd ^= 1) {
       if (D == 128 && odd == 0)
         for (; kt >= whole && kt + 1 < cut; kt += 2) {
@@ -995,6 +1013,10 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
   if (p_total > 0) {
     p_runs = a.runs;
     if (s_total > 0) {
+      // By measurement; us with 0.15 / 0.25 / 0.4 of fp8: 64 rows, 64 heads over 8, 4,000
+      // shared, up to 3,000 more 55.4 / 52.4 / 66.2; of 60,000 and 4,000 183.5 / 184.2 /
+      // 206. bf16, 0.18 / 0.3 / 0.5: 64 rows, 2,048 and 2,000 64.1 / 62.4 / 73.6; 256 rows,
+      // 8,000 and 600 99.1 / 98.5 / 113; 512 rows, 500 and 500 142.6 / 141.4 / 191.7.
       const float p_cost = p_total, s_cost = s_total * (FP8 ? 0.25f : 0.3f);
       p_runs = uniform((int)(a.runs * (p_cost / (p_cost + s_cost)) + 0.5f));
       p_runs = min(max(p_runs, 1), a.runs - 1);
@@ -1002,7 +1024,7 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
     // Where there are no more item tiles than workgroups, each has a run of one item
     // tile's key tiles, the shortest length that this gives for all; otherwise equal runs
     // of the list of all of them. A run's begin and end cost as much as four key tiles.
-    per = uniform(max((p_total + p_runs - 1) / p_runs, p_total >= 64 ? 2 : 1));
+    per = uniform((p_total + p_runs - 1) / p_runs);
     apart = tiles <= p_runs;
     int used = (p_total + per - 1) / per;
     while (apart) {  // ends where per is the longest group's at the latest
@@ -1116,7 +1138,9 @@ extern "C" void launch_shared_prefix(const SharedPrefix* a, bool fp8, hipStream_
   if (a->D == 128) fp8 ? run(shared_prefix_kernel<128, true>)
                        : run(shared_prefix_kernel<128, false>);
   else fp8 ? run(shared_prefix_kernel<64, true>) : run(shared_prefix_kernel<64, false>);
-  // few rows: four waves each, which share its parts
+  // Few rows: four waves each, which share its parts. One / four, us of the call: 8
+  // rows of 32 heads over 100,000 tokens 95.7 / 90.3, 256 over 8,000 98.6 / 108.6, 128 rows
+  // of 64 heads over 256 tokens 26.0 / 34.6.
   const bool wide = a->B * a->Hq <= 1024;
   const dim3 heads(wide ? a->Hq : (a->Hq + 3) / 4, a->B);
   auto join = [&](auto kernel) { kernel<<<heads, 256, 0, stream>>>(*a); };
