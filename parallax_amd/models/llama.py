@@ -218,7 +218,8 @@ class LlamaAttention(nn.Module):
                 q, k_cache, v_cache, meta.block_tables, meta.seq_lens,
                 meta.query_lens, self.scale, self.sliding_window, sinks=sinks,
             )
-        elif meta.prefix_group is not None:
+        elif meta.prefix_group is not None and self.sliding_window <= 0:
+            # a window leaves little of a prefix: one launch is faster than two
             attn = ops.shared_prefix_attention_decode(
                 q, k_cache, v_cache, meta.block_tables, meta.seq_lens,
                 meta.prefix_group, meta.prefix_lens, self.scale, self.sliding_window,

@@ -341,6 +341,8 @@ class Engine:
                 isinstance(m, LlamaAttention) for m in self.model.modules()):
             raise ValueError(f"shared_prefix_attention: {self.cfg.architecture} has "
                              "layers without it")
+        if all(m.sliding_window > 0 for m in modules):
+            raise ValueError("shared_prefix_attention: all layers have windows")
         if not self.args.enable_prefix_cache:
             raise ValueError("shared_prefix_attention needs the prefix cache")
         if self.device.type == "cuda" and (

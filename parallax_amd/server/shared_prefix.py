@@ -22,8 +22,10 @@ from .kv_cache import KVCacheSpec
 # 18.6 shared, 17.5 plain; over 2,048 (126 MB) 19.0, 20.8; 64 rows over 1,024 (264 MB)
 # 30.2, 35.9; over 2,048 (528 MB) 31.7, 47.1; 256 over 8,000 (8.4 GB) 99.6, 425. 64 over 8
 # of 64, 64 rows over 2,048 (264 MB) 23.3, 29.3; 14 over 2 of 64, 256 over 2,048 (267 MB)
-# 22.6, 28.0.
-LEAST_BYTES = 256 << 20
+# 22.6, 28.0. Whole decode steps, four layers of 8B's sizes, ms: 64 requests behind 1,024
+# shared tokens (264 MB) 1.006 shared, 0.996 plain; 2,048 (528 MB) 1.008, 1.061; 128 behind
+# 4,000 (2 GB) 1.497, 1.850; 256 behind 8,000 (8.4 GB) 2.460, 3.984.
+LEAST_BYTES = 384 << 20
 MAX_GROUPS = 32    # as many as a graph's buffers hold; those that save most are kept
 MAX_ROWS = 4096    # the kernel's own limit
 

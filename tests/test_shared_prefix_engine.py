@@ -188,6 +188,9 @@ def test_refusals():
         _engine(_cfg(), fused_head_norms=True)
     with pytest.raises(ValueError, match="no norms of single heads"):
         _engine(_cfg(qk_norm=True, qk_norm_full=True), fused_head_norms=True)
+    with pytest.raises(ValueError, match="all layers have windows"):
+        _engine(_cfg(sliding_window=8, layer_types=["sliding_attention"] * 2),
+                shared_prefix_attention=True)
     with pytest.raises(ValueError, match="needs the prefix cache"):
         _engine(_cfg(), shared_prefix_attention=True, enable_prefix_cache=False)
 

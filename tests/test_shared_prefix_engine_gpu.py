@@ -23,6 +23,9 @@ FAMILIES = {
     "llama": {"architectures": ["LlamaForCausalLM"], "model_type": "llama"},
     "wide": {"architectures": ["LlamaForCausalLM"], "model_type": "llama",
              "head_dim": 128},
+    "windows": {"architectures": ["LlamaForCausalLM"], "model_type": "llama",
+                "sliding_window": 48,
+                "layer_types": ["sliding_attention", "full_attention"]},
     "qwen3": {"architectures": ["Qwen3ForCausalLM"], "model_type": "qwen3"},
 }
 HEADS = [[(7 * i + 3 + 50 * g) % 500 for i in range(150 + 60 * g)] for g in range(2)]
@@ -75,6 +78,7 @@ def _apart(a, b):
     ("llama", False, False, "auto"),
     ("llama", False, True, "fp8"),
     ("wide", False, True, "auto"),
+    ("windows", False, True, "auto"),
     ("qwen3", False, True, "auto"),
     ("qwen3", True, True, "auto"),
     ("qwen3", True, False, "fp8"),
