@@ -368,9 +368,11 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     auto top_of = [&](float x) INL {
       return over_halves(x, [](float p, float q) { return fmaxf(p, q); }) * c;
     };
-    // rescaled when a maximum moved: its own weight is then 1, without error
+    // Rescaled when a maximum moved by more than 8: weights up to 2^8 are rounded and
+    // summed as well as those up to 1. At any move, which 32 items have in three turns of
+    // four, 64 rows over 60,000 tokens take 154 us.
     auto raise = [&]() INL {
-      if (__any(mx > m)) {
+      if (__any(mx > m + 8.f)) {
         const float m2 = fmaxf(m, mx);
         const float f = __builtin_amdgcn_exp2f(m - m2);
         m = m2;
