@@ -99,36 +99,44 @@ def find_shared_prefixes(tables: Sequence, seq_lens: Sequence[int],
 
 
 class SharedPrefixes:
-    """find_shared_prefixes() of the batch at hand, found again when its rows change, and
-    nothing where too little would be saved."""
+    """find_shared_prefixes() of the batch at hand, and nothing where too little would be
+    saved: found again when the rows change, and kept for the last BATCHES batches, which
+    a pipeline's stages go through in turn."""
+
+    BATCHES = 8
 
     def __init__(self, spec: KVCacheSpec, least_bytes: int = LEAST_BYTES):
         token = 2 * spec.num_kv_heads * spec.head_dim * spec.dtype.itemsize
         self.least_tokens = -(-least_bytes // token)
         self.block_size = spec.block_size
-        self._tables: List[List[int]] = []
-        self._pages: List[np.ndarray] = []  # the same tables, which take long to convert
-        self._found = None
+        # of each batch its tables, the same as arrays (which take long to convert) and
+        # what was found; the latest first
+        self._batches: List[tuple] = []
 
     def find(self, tables, seq_lens):
         """(groups, lengths) as above, or None. A table only grows while its request
         lives, so the same tables share the same pages; held, none is taken for another."""
-        if len(tables) != len(self._tables) or any(
-                a is not b for a, b in zip(tables, self._tables)):
-            known = {id(t): p for t, p in zip(self._tables, self._pages)}
-            self._pages = [self._extended(known.get(id(t)), t) for t in tables]
-            self._tables, self._found = list(tables), None
-            if len(tables) <= MAX_ROWS:
-                groups, lens = find_shared_prefixes(self._pages, seq_lens,
-                                                    self.block_size)
-                rows = [0] * len(lens)
-                for g in groups:
-                    if g >= 0:
-                        rows[g] += 1
-                if sum(t * (n - 1) for t, n in zip(lens, rows)) >= max(
-                        1, self.least_tokens):
-                    self._found = groups, lens
-        return self._found
+        for i, batch in enumerate(self._batches):
+            if len(batch[0]) == len(tables) and all(
+                    a is b for a, b in zip(batch[0], tables)):
+                if i:
+                    self._batches.insert(0, self._batches.pop(i))
+                return batch[2]
+        known = {id(t): p for kept, pages, _ in reversed(self._batches)
+                 for t, p in zip(kept, pages)}
+        pages = [self._extended(known.get(id(t)), t) for t in tables]
+        found = self._worthwhile(pages, seq_lens) if len(tables) <= MAX_ROWS else None
+        self._batches = [(list(tables), pages, found)] + self._batches[:self.BATCHES - 1]
+        return found
+
+    def _worthwhile(self, pages, seq_lens):
+        groups, lens = find_shared_prefixes(pages, seq_lens, self.block_size)
+        rows = [0] * len(lens)
+        for g in groups:
+            if g >= 0:
+                rows[g] += 1
+        saved = sum(t * (n - 1) for t, n in zip(lens, rows))
+        return (groups, lens) if saved >= max(1, self.least_tokens) else None
 
     @staticmethod
     def _extended(pages, table) -> np.ndarray:

@@ -114,6 +114,14 @@ def test_found_again_only_for_other_rows():
     a.append(7)
     assert s.find([a, b], [13, 10]) is found
     assert s.find([a, list(b)], [13, 10]) is not found
+    assert s.find([a, b], [13, 10]) is found      # two batches in turn
+    assert s.find([b, a], [10, 13]) == found
+    c = [1, 2, 5]
+    for _ in range(20):
+        s.find([list(a), c], [13, 9])
+    assert len(s._batches) == s.BATCHES
+    again = s.find([a, b], [13, 10])
+    assert again is not found and again == found
     assert SharedPrefixes(spec, least_bytes=8 * token + 1).find([a, b], [13, 9]) is None
     assert SharedPrefixes(spec, least_bytes=0).find([a, [9]], [13, 3]) is None
 
