@@ -132,6 +132,7 @@ def test_far_slots():
 
 
 @pytest.mark.parametrize("T", [8, 1200])
+@torch.inference_mode()  # engines capture in it: outside, none could behind them
 def test_captured(T):
     """A captured call follows its inputs, on a stream of its own."""
     s = store_inputs(T, 8, 2, 128, 64, 32, True, slots=torch.arange(T))

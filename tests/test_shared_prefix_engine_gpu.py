@@ -2,6 +2,8 @@
 GPU, against the fp32 engine on the CPU fed the same tokens: prompts of a common head,
 steps replayed and not, rows that leave, a second batch over other groups."""
 
+import gc
+
 import pytest
 import torch
 
@@ -29,6 +31,14 @@ FAMILIES = {
     "qwen3": {"architectures": ["Qwen3ForCausalLM"], "model_type": "qwen3"},
 }
 HEADS = [[(7 * i + 3 + 50 * g) % 500 for i in range(150 + 60 * g)] for g in range(2)]
+
+
+@pytest.fixture(autouse=True)
+def engines_end_with_their_test():
+    # graphs captured in inference mode leave torch's generator state such that none can
+    # be captured outside of it while they live, and an engine lives on in cycles
+    yield
+    gc.collect()
 
 
 def _prompts(groups):

@@ -173,6 +173,7 @@ def test_far_pages():
     assert_attended(prefix_call(far, s, "cuda"), want)
 
 
+@torch.inference_mode()  # engines capture in it: outside, none could behind them
 def test_captured():
     """Two captured calls follow lengths, groups and tables, also between eager ones."""
     B = 24
@@ -317,6 +318,7 @@ def test_any(seed):
                         q_gap=r.choice([0, 8])), **kw)
 
 
+@torch.inference_mode()  # engines capture in it: outside, none could behind them
 def test_two_at_once():
     """Calls on two streams and graphs replayed on both, each with results of its own."""
     a = prefix_inputs(8, 2, 64, 16, ODD, [200, 129])
