@@ -27,16 +27,16 @@
 //
 // What bounds it, replayed in graphs, 32 query heads over 8 of 128 in bf16 unless said:
 // Long prefixes by the products with the softmax's instructions beside them, and by the
-// card's power: 64 rows, 64 heads over 8, 60,000 shared tokens 146 us, of which this
-// launch has 135, 930 TFLOP/s, where a product of 8192^3 reaches 1,213; at 1.9 GHz matrix
-// and vector units are busy 46% and 40% of the time, and neither the order of a turn nor
-// how far ahead operands are read moves it. Of an fp8 cache 143, 178 with up to 4,000 more
+// card's power: 64 rows, 64 heads over 8, 60,000 shared tokens 152 us, of which this
+// launch has 141, 890 TFLOP/s, where a product of 8192^3 reaches 1,213; at 1.9 GHz matrix
+// and vector units are busy 42% and 44% of the time, and neither the order of a turn nor
+// how far ahead operands are read moves it. Of an fp8 cache 149, 181 with up to 4,000 more
 // tokens a row. Suffixes by the stream of their keys and values: 8 rows over 100,000, where
-// the prefix is little more than a stream too, 88 us, 4.7 TB/s. Both together: 256 rows
-// over 8,000, up to 600 of their own, 97, of which the prefix alone is 53 and the rest
+// the prefix is little more than a stream too, 91 us, 4.5 TB/s. Both together: 256 rows
+// over 8,000, up to 600 of their own, 98, of which the prefix alone is 57 and the rest
 // alone 89. Small batches by waits in a row, of lengths, lists, page numbers, a tile, and
 // by the second launch: 4 rows over 700 tokens, 14 heads over 2 of 64, 10.6; 16 rows over
-// 500, up to 300 of their own, 14.8, where paged_decode.hip starts with 6. The second
+// 500, up to 300 of their own, 15, where paged_decode.hip starts with 6. The second
 // launch is 4 to 10 of each, 9 where it reads the 34 MB that 512 workgroups leave.
 //
 // Keys and values of 16-bit caches go to LDS by buffer instructions: behind global ones
@@ -370,11 +370,12 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     auto top_of = [&](float x) INL {
       return over_halves(x, [](float p, float q) { return fmaxf(p, q); }) * c;
     };
-    // Rescaled when a maximum moved by more than 8: weights up to 2^8 are rounded and
-    // summed as well as those up to 1. At any move, which 32 items have in three turns of
-    // four, 64 rows over 60,000 tokens take 157 us, here 149.
+    // Rescaled whenever a maximum moved, which 32 items have in three turns of four: the
+    // largest weight is then 1, without error. Only at moves by more than 2^8, 64 rows
+    // over 60,000 tokens take 149 us for 157, but the error against 64 bits goes from 1.8e-3
+    // of the result, of which its own rounding has 1.6e-3, to 2.3e-3.
     auto raise = [&]() INL {
-      if (__any(mx > m + 8.f)) {
+      if (__any(mx > m)) {
         const float m2 = fmaxf(m, mx);
         const float f = __builtin_amdgcn_exp2f(m - m2);
         m = m2;
@@ -604,8 +605,8 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
             bf16x8v, __builtin_bit_cast(u32x4v, qf[s]) ^ 0x80008000u);
     // Whole turns apart only of 128: with heads of 64 the compiler runs out of the 168
     // registers of three workgroups a CU. 64 heads over 8, without / with, us: 100 rows in
-    // five groups over 5,000 tokens 37.8 / 39.1; of an fp8 cache 16 rows over 500 14.3 /
-    // 15.0, 64 over 2,000 22.3 / 23.2, 256 over 8,000 67.6 / 64.6.
+    // five groups over 5,000 tokens 37.7 / 39.1; of an fp8 cache 16 rows over 500 14.4 /
+    // 15.1, 64 over 2,000 22.1 / 23.1, 256 over 8,000 70.7 / 67.3.
     for (int kt = k0, odd = 0; kt <= k1; ++kt, odd ^= 1) {
       if (D == 128 && odd == 0)
         for (; kt >= whole && kt + 1 < cut; kt += 2) {
@@ -1019,9 +1020,9 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
     p_runs = a.runs;
     if (s_total > 0) {
       // By measurement; us with 0.15 / 0.25 / 0.4 of fp8: 64 rows, 64 heads over 8, 4,000
-      // shared, up to 3,000 more 55.4 / 52.2 / 60.3; of 60,000 and 4,000 178 / 178 / 190.
-      // bf16, 0.18 / 0.3 / 0.5: 64 rows, 2,048 and 2,000 64.6 / 62.8 / 71.1; 256 rows,
-      // 8,000 and 600 98.1 / 97.3 / 102.6; 512 rows, 500 and 500 142.7 / 142.0 / 165.4.
+      // shared, up to 3,000 more 54.8 / 52.2 / 61.5; of 60,000 and 4,000 180 / 181 / 194.
+      // bf16, 0.18 / 0.3 / 0.5: 64 rows, 2,048 and 2,000 64.1 / 62.5 / 71.4; 256 rows,
+      // 8,000 and 600 97.0 / 97.9 / 102.8; 512 rows, 500 and 500 142.7 / 141.7 / 168.4.
       const float p_cost = p_total, s_cost = s_total * (FP8 ? 0.25f : 0.3f);
       p_runs = uniform((int)(a.runs * (p_cost / (p_cost + s_cost)) + 0.5f));
       p_runs = min(max(p_runs, 1), a.runs - 1);
@@ -1144,8 +1145,8 @@ extern "C" void launch_shared_prefix(const SharedPrefix* a, bool fp8, hipStream_
                        : run(shared_prefix_kernel<128, false>);
   else fp8 ? run(shared_prefix_kernel<64, true>) : run(shared_prefix_kernel<64, false>);
   // Few rows: four waves each, which share its parts. One / four, us of the call: 8
-  // rows of 32 heads over 100,000 tokens 93.2 / 88.0, 256 over 8,000 97.3 / 106.1, 128 rows
-  // of 64 heads over 256 tokens 25.9 / 34.4.
+  // rows of 32 heads over 100,000 tokens 96.6 / 91.2, 256 over 8,000 98.6 / 108.6, 128 rows
+  // of 64 heads over 256 tokens 26.0 / 34.6.
   const bool wide = a->B * a->Hq <= 1024;
   const dim3 heads(wide ? a->Hq : (a->Hq + 3) / 4, a->B);
   auto join = [&](auto kernel) { kernel<<<heads, 256, 0, stream>>>(*a); };
