@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void head_norm_store_kernel(const HeadNormStor
   __syncthreads();
   if (!on) return;
   const int64_t slot = kind == 0 ? 0 : a.slots[t];
-  if (slot < 0 || slot >= a.num_slots) return;
+  if (kind > 0 && (slot < 0 || slot >= a.num_slots)) return;
   const int64_t row = (slot / a.BS) * a.Hk + h;
   const int in = (int)(slot % a.BS);
   const int p = a.positions[t], half = a.rot / 2;
