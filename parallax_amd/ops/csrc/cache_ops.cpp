@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <initializer_list>
@@ -212,7 +213,8 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   a.q_stride = q.stride(0);
   a.scale = (float)(fp8 ? scale * k_scale : scale);
   a.v_scale = fp8 ? (float)v_scale : 1.f;
-  a.softcap = (float)softcap;
+  // within fp32: below, nothing is left of a score; above, all of it
+  a.softcap = softcap > 0 ? (float)std::clamp(softcap, 1e-30, (double)FLT_MAX) : 0.f;
   a.window = sliding_window > 0 ? (int)std::min<int64_t>(sliding_window, INT_MAX) : 0;
   int tiles;
   shared_prefix_plan(a.B, a.N, a.Hq, a.Hk, a.D, &a.runs, &tiles);

@@ -95,12 +95,27 @@ DEVINL int page_at(const SharedPrefix& a, int entry) {
   return min(max(entry, 0), a.num_pages - 1);
 }
 
-// log2(e) cap tanh(x) of x = y / cap, y2 = 2 log2(e) x: off by some 2^-22 of the cap,
-// also where x is small, and that is what a weight's error goes by
-DEVINL float capped(float y2, float cap) {
-  const float e = __builtin_amdgcn_exp2f(y2);
-  return cap * kLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e));
-}
+// log2(e) cap tanh(y / cap) of a product s, whose score is y: y2 = 2 log2(e) y / cap,
+// flat = log2(e) y. From |y| = cap / 4 on by the exponential, off by some 2^-22 of the cap;
+// below, where that would be more than a weight may be off by, by tanh's series, the next
+// term of which is 2^-26 of the result. What it multiplies is y itself, so that caps far
+// above the scores leave them as they are.
+struct Cap {
+  float flat, twice, cap;  // log2(e) |scale|, 2 log2(e) |scale| / cap, log2(e) cap
+  DEVINL explicit Cap(const SharedPrefix& a)
+      : flat(kLog2e * fabsf(a.scale)),
+        twice(2.f * kLog2e * fabsf(a.scale) / fmaxf(a.softcap, 1e-30f)),
+        cap(kLog2e * a.softcap) {}
+  DEVINL float operator()(float s) const {
+    constexpr float t = 0.25f / (kLog2e * kLog2e);  // of y2^2: x^2
+    const float y2 = s * twice, x2 = y2 * y2 * t;
+    const float e = __builtin_amdgcn_exp2f(y2);
+    const float bent = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e));
+    const float p = fmaf(fmaf(fmaf(fmaf(62.f / 2835, x2, -17.f / 315), x2, 2.f / 15), x2,
+                              -1.f / 3), x2, 1.f);
+    return x2 < 0.0625f ? s * flat * p : bent;
+  }
+};
 
 // n / g of n below 2^20, exactly: n + 1/2 is 1/32 at least from where a quotient changes
 DEVINL int over(int n, int g) {
@@ -235,7 +250,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   };
   // above 0 also for a scale of 0: hidden scores are multiplied by it too
   const float c = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1e-20f);
-  const float cap2 = 2.f * kLog2e * fabsf(a.scale) / fmaxf(a.softcap, 1e-30f);
+  const Cap capped(a);
 
   int done = 0;
   while (todo > 0) {
@@ -489,7 +504,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              s0[t][e] = capped(s0[t][e] * cap2, a.softcap);
+              s0[t][e] = capped(s0[t][e]);
         }
         if (base + SP_KT > P || base < lo_most) {
           int begin = lo - base - 8 * half;  // tokens [begin, begin + count) are seen
@@ -709,7 +724,7 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       FP8 ? lds_at(Vt) + l15 * VB + ((l4 >> 1) ^ swz_v<FP8>(l15)) * 16 + (l4 & 1) * 8
           : lds_at(Vt) + l15 * VB + (l4 ^ swz_v<FP8>(l15)) * 16;
   const float c = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1e-20f);
-  const float cap2 = 2.f * kLog2e * fabsf(a.scale) / fmaxf(a.softcap, 1e-30f);
+  const Cap capped(a);
 
   // Rows 64 at a time, one a lane: where its own tokens begin and end.
   int rows0 = -64, row_lo = 0, row_end = 0;
@@ -851,7 +866,7 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     if (a.softcap > 0.f) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        s[e >> 2][e & 3] = capped(s[e >> 2][e & 3] * cap2, a.softcap);
+        s[e >> 2][e & 3] = capped(s[e >> 2][e & 3]);
     }
     const bool cut = tok + KT > L || tok < lo;
     if (cut) {

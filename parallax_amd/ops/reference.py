@@ -272,8 +272,9 @@ def shared_prefix_attention_decode(
         v = v_cache[page, :, :, tok % block_size].float() * v_scale
         x = q[b].float().view(Hk, Hq // Hk, D)
         z = torch.einsum("hgd,lhd->hgl", x, k).reshape(Hq, -1) * scale
-        if softcap > 0:
-            z = softcap * torch.tanh(z / softcap)
+        if softcap > 0:  # 64 bits: z over a large cap is no number of 32
+            cap = min(max(softcap, 1e-30), 1e38)
+            z = (cap * torch.tanh(z.double() / cap)).float()
         if sinks is not None:
             z = torch.cat([z, sinks.float().unsqueeze(-1)], dim=-1)
         p = torch.softmax(z, dim=-1)[:, : len(tok)].view(Hk, Hq // Hk, -1)

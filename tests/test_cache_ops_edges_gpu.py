@@ -28,3 +28,25 @@ def test_store_without_pages(T, D, rot, head_gap):
                      slots=torch.arange(T))
     torch.full((T, 4, D), NAN, dtype=torch.bfloat16, device="cuda")  # what `out` finds
     assert_stored(call(STORE, s, "cuda"), *store_oracle(s, True))
+
+
+CAPS = [1e3, 1e5, 1e8, 1e30, 3e38, 1e300]
+
+
+@pytest.mark.parametrize("softcap", CAPS)
+@pytest.mark.parametrize("D,fp8", [(64, False), (64, True), (128, False), (128, True)])
+def test_large_caps(softcap, D, fp8):
+    """Caps far above the scores leave them as they are."""
+    s = prefix_inputs(8, 2, D, 32, ODD, [200, 129], fp8, seed=D)
+    for scale in (None, -0.3):
+        got = prefix_call(ATTEND, s, "cuda", softcap=softcap, scale=scale)
+        assert_attended(got, prefix_oracle(s, softcap=softcap, scale=scale))
+
+
+@pytest.mark.parametrize("softcap", [1e-300, 1e-20, 1e-3, 0.5, 3.0, 8.0, 20.0])
+def test_caps_about_the_scores(softcap):
+    """Scores on both sides of where a cap begins to bend them, and caps that leave
+    nothing of them."""
+    s = prefix_inputs(8, 2, 64, 32, ODD, [200, 129], seed=3)
+    got = prefix_call(ATTEND, s, "cuda", softcap=softcap)
+    assert_attended(got, prefix_oracle(s, softcap=softcap))
