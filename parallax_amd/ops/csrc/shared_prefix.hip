@@ -1119,7 +1119,7 @@ __global__ __launch_bounds__(256) void shared_prefix_join_kernel(const SharedPre
       for (int j = 0; j < AHEAD; ++j) {
         const int i = j0 + first + j * W * GROUPS;
         const float y = __shfl(w, min(i, n - 1), WAVE_SIZE);
-        s += x[j] * (i < n ? y : 0.f);
+        if (i < n) s += x[j] * y;  // else a part again: infinity times 0 is no number
       }
       if (j0 + AHEAD * W * GROUPS < n)
 #pragma unroll

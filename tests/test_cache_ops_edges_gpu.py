@@ -50,3 +50,41 @@ def test_caps_about_the_scores(softcap):
     s = prefix_inputs(8, 2, 64, 32, ODD, [200, 129], seed=3)
     got = prefix_call(ATTEND, s, "cuda", softcap=softcap)
     assert_attended(got, prefix_oracle(s, softcap=softcap))
+
+
+def assert_same_numbers(got, oracle):
+    """Infinities and NaN where the oracle has them, and what is left as ever. -> how
+    many values and rows have some."""
+    want, size = oracle
+    x = got.cpu().double()
+    assert torch.equal(x.isnan(), want.isnan())
+    assert torch.equal(x.isinf(), want.isinf())
+    assert torch.equal(x[x.isinf()], want[want.isinf()])
+    none = ~torch.isfinite(want)
+    assert_attended(x.masked_fill(none, 0.0),
+                    (want.masked_fill(none, 0.0), size.masked_fill(none, 0.0)))
+    return int(none.sum()), int(none.any(-1).any(-1).sum())
+
+
+def put_value(s, row, token, head, d, value):
+    BS = s["kc"].shape[2]
+    page = int(s["tables"][row, token // BS])
+    s["vc"][page, head, d, token % BS] = value
+
+
+@pytest.mark.parametrize("value", [NAN, INF])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_that_are_no_numbers(D, value):
+    """Of a prefix and of a row's own tokens, in rows of many parts and of one: one value
+    a head is none, the others are as ever."""
+    rows = [(0, 3000 + 70 * i) for i in range(5)] + [(-1, 5000), (-1, 33), (0, 3000)]
+    s = prefix_inputs(8, 2, D, 32, rows, [3000], seed=D)
+    put_value(s, 0, 17, 0, 5, value)
+    put_value(s, 2, 3100, 1, 9, value)
+    put_value(s, 5, 4000, 0, 30, value)
+    put_value(s, 6, 32, 1, 31, value)
+    got = prefix_call(ATTEND, s, "cuda")
+    values, _ = assert_same_numbers(got, prefix_oracle(s))
+    # head 0 of the six rows of the group, head 1 of row 2, one each of rows 5 and 6: four
+    # query heads a head
+    assert values == 4 * (6 + 1 + 1 + 1)
