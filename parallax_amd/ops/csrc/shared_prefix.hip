@@ -139,7 +139,7 @@ struct Lists {
   int* prefix;      // the groups' lengths
   int* count;       // rows of a group
   int* low;         // where the first window of a group's rows begins
-  int* rows;        // of an item tile; [SP_ITEMS]: its group's first row
+  int* rows;        // of an item tile; [SP_ITEMS]: its group's first row, then a key tile
   int2* span;       // of the first SP_SPANS rows: where a row's own tokens begin and end
   int16_t* member;  // a row's group, -1: none
   int* units;       // a row's suffix tiles; here the tiles come to lie
@@ -268,6 +268,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     const int r1 = uniform(over(min((tile + 1) * SP_ITEMS, n_items) - 1, G));
     __syncthreads();  // the buffers and the list are free
     if (wid == 0) {
+      if (lane == 0) w.rows[SP_ITEMS + 1] = -1;
       int rank = 0;
       for (int b0 = 0; b0 < a.B && rank <= r1; b0 += 64) {
         const bool is = b0 + lane < a.B && w.member[b0 + lane] == g;
@@ -297,6 +298,15 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     }
     lo_most = uniform(lo_most);
     const int lo_least = uniform(w.low[g]);
+    int lo_last = 0;  // of the tile's rows
+    if (a.window > 0) {
+      for (int i = lane; i <= r1 - r0; i += 64)
+        lo_last = max(lo_last, window_start(a, length(a, w.rows[i])));
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1)
+        lo_last = max(lo_last, __shfl_xor(lo_last, o, WAVE_SIZE));
+    }
+    lo_last = uniform(lo_last);
     const int part0 = apart ? run : run + tile0 + tile;
 
     if (k0 == kb && half == 0 && on)
@@ -433,6 +443,50 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       }
     };
 
+    // What one item sees and another's window hides must stay, and the other's weight 0
+    // times NaN or infinity would be NaN. A tile that has such values loses them here, and
+    // the items that see them get them as they are, behind their rescaling.
+    auto part_numbers = [&](int base, int tag, uint16_t* Vl) INL {
+      u32x4v* const mine = reinterpret_cast<u32x4v*>(Vl + wid * GROUP);
+      int* const found = w.rows + SP_ITEMS + 1;
+      uint32_t any = 0;
+#pragma unroll 1
+      for (int i = lane; i < GROUP / 8; i += 64)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) any |= (mine[i][j] & 0x7f807f80u) + 0x00800080u;
+      if ((any & 0x80008000u) != 0) *found = tag;
+      __syncthreads();
+      if (*found != tag) return;
+      raise();
+#pragma unroll 1
+      for (int tok = 0; tok < SP_KT; ++tok) {
+        const bool seen = base + tok >= lo && base + tok < P;
+        // value d = 32 t + 8 i + 4 half + e of the token, its chunks exchanged for odd i
+        const uint16_t* at = Vl + (tok >> 4) * GROUP + half * 64 + (tok & 7);
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int i = e >> 2;
+            const uint16_t x =
+                at[(32 * t + 8 * i + (e & 3)) * 16 + ((tok & 8) ^ (i & 1) * 8)];
+            if (seen && (x & 0x7f80) == 0x7f80) o[t][e] += bf16_bits_to_f32(x);
+            if ((e & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int i = lane; i < GROUP / 8; i += 64) {
+        u32x4v f = mine[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          f[j] &= ((f[j] & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) |
+                  ((f[j] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+        mine[i] = f;
+      }
+      __syncthreads();
+    };
+
     // A turn takes the scores of tile kt and the weights and values of the tile before,
     // which depend on nothing of this turn. It copies K of the next tile and V of its
     // own. Any turn: also the first and the last, a softcap, a mask. `odd` (0 or 1): of
@@ -462,6 +516,9 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
         clean((kt - 1) * SP_KT, Vl);
         __syncthreads();
       }
+      const int prev = (kt - 1) * SP_KT;
+      if (!first && prev < lo_last && prev + SP_KT > lo_least)
+        part_numbers(prev, kt, Vl);
       // operands are read AHEAD products early here too
       constexpr int AHEAD = 4;
       bf16x8v fr[AHEAD];
@@ -584,8 +641,8 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       }
     };
 
-    const int whole = max(max(k0 + 1, (lo_least + SP_KT - 1) / SP_KT + 1),
-                          (lo_most + SP_KT - 1) / SP_KT);
+    // the same for all waves where a turn has more barriers than one
+    const int whole = max(k0 + 1, (lo_last + SP_KT - 1) / SP_KT + 1);
     const int cut = wave_on && a.softcap <= 0.f ? min(k1, P / SP_KT) : 0;
 
     // The first turn's K, and behind it what that turn would ask for: the buffers are

@@ -88,3 +88,23 @@ def test_values_that_are_no_numbers(D, value):
     # head 0 of the six rows of the group, head 1 of row 2, one each of rows 5 and 6: four
     # query heads a head
     assert values == 4 * (6 + 1 + 1 + 1)
+
+
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("Hq,Hk,D,BS,fp8", [
+    (8, 1, 64, 16, False), (8, 2, 128, 32, False), (3, 3, 128, 64, False),
+    (16, 1, 128, 32, True), (6, 2, 64, 64, True),
+])
+def test_windows_over_no_numbers(Hq, Hk, D, BS, fp8, value):
+    """A shared token that one row's window hides and another's does not: only the rows
+    that see it get its NaN or infinity."""
+    rows = [(0, 300 + 3 * i) for i in range(33)] + [(0, 900), (-1, 170), (0, 320)]
+    s = prefix_inputs(Hq, Hk, D, BS, rows, [250], fp8, seed=D + BS)
+    put = [(152, 0, 5), (200, Hk - 1, D - 1), (201, Hk - 1, 0), (231, 0, 33),
+           (249, 0, 40)]
+    for token, head, d in put:
+        put_value(s, 0, token, head, d, value)
+    want = prefix_oracle(s, sliding_window=150)
+    got = prefix_call(ATTEND, s, "cuda", sliding_window=150)
+    values, seen_by = assert_same_numbers(got, want)
+    assert 0 < values and 30 < seen_by < len(rows)
