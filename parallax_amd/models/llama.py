@@ -169,6 +169,14 @@ class LlamaAttention(nn.Module):
                 torch.empty(self.num_heads, dtype=torch.float32), requires_grad=False
             )
 
+    def fuses_head_norms(self) -> bool:
+        """Whether one launch norms the heads, for norms that are no more than RMSNorm:
+        hooks and forwards of others see the rows."""
+        return self.fused_head_norms and self.qk_norm and not self.qk_norm_full and (
+            plain_call(self.q_norm, RMSNorm.forward)
+            and plain_call(self.k_norm, RMSNorm.forward)
+            and self.q_norm.eps == self.k_norm.eps)
+
     def forward(self, x: torch.Tensor, meta: ForwardMeta, rope_cache: torch.Tensor):
         return self.attend(self.qkv_proj(x), x, meta, rope_cache)
 
@@ -185,7 +193,7 @@ class LlamaAttention(nn.Module):
         v = v.view(T, self.num_kv_heads, self.head_dim)
         k_cache, v_cache = meta.kv_cache.layer(self.local_layer_idx)
         sinks = self.sinks.float() if self.sinks is not None else None
-        fused = self.fused_head_norms and self.qk_norm and not self.qk_norm_full
+        fused = self.fuses_head_norms()
         if fused:
             q = ops.qk_norm_rope_and_cache(
                 q, k, v, self.q_norm.weight, self.k_norm.weight, self.q_norm.eps,

@@ -21,3 +21,45 @@ def test_caps(softcap):
     s = prefix_inputs(4, 2, 64, 16, ROWS, [20, 32])
     got = prefix_call(ATTEND, s, "cpu", softcap=softcap)
     assert_attended(got, prefix_oracle(s, softcap=softcap), weights=0.0)
+
+
+@pytest.mark.parametrize("name", ["q_norm", "k_norm"])
+def test_hooks_of_head_norms_run(name):
+    """A hook on a head's norm sees its rows and may change them, fused or not."""
+    cfg = _cfg(qk_norm=True)
+    outs, calls = [], []
+    for fused in (False, True):
+        eng = _engine(cfg, fused_head_norms=fused)
+        for layer in eng.model.layers:
+            getattr(layer.self_attn, name).register_forward_hook(
+                lambda m, x, y: calls.append(fused) or -2 * y)
+        outs.append(_generate(eng))
+    assert outs[0] == outs[1] and calls.count(True) == calls.count(False) > 0
+
+
+def test_other_head_norms_run():
+    """A module in a norm's place, and norms of two epsilons, are called."""
+    from parallax_amd.models.llama import RMSNorm
+
+    class Shifted(RMSNorm):
+        def forward(self, x):
+            return super().forward(x) + 1
+
+    def shift(attn):
+        old = attn.k_norm
+        attn.k_norm = Shifted(attn.head_dim, old.eps)
+        attn.k_norm.weight = old.weight
+
+    def loosen(attn):
+        attn.k_norm.eps = 3.0
+
+    cfg = _cfg(qk_norm=True)
+    plain = _generate(_engine(cfg))
+    for change in (shift, loosen):
+        outs = []
+        for fused in (False, True):
+            eng = _engine(cfg, fused_head_norms=fused)
+            for layer in eng.model.layers:
+                change(layer.self_attn)
+            outs.append(_generate(eng))
+        assert outs[0] == outs[1] != plain
