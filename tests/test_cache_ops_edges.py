@@ -63,3 +63,14 @@ def test_other_head_norms_run():
                 change(layer.self_attn)
             outs.append(_generate(eng))
         assert outs[0] == outs[1] != plain
+
+
+def test_scales_of_a_bf16_cache():
+    """Scales are those of fp8 caches; a bf16 one holds its values as they are."""
+    s = prefix_inputs(4, 2, 64, 16, ROWS, [20, 32])
+    want = prefix_call(ATTEND, s, "cpu")
+    assert torch.equal(prefix_call(ATTEND, {**s, "scales": (0.5, 0.25)}, "cpu"), want)
+    s = store_inputs(9, 4, 2, 64, 64, 16)
+    for got, want in zip(call(STORE, s, change=dict(k_scale=0.5, v_scale=0.25)),
+                         call(STORE, s)):
+        assert torch.equal(got, want)

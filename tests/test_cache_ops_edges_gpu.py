@@ -108,3 +108,14 @@ def test_windows_over_no_numbers(Hq, Hk, D, BS, fp8, value):
     got = prefix_call(ATTEND, s, "cuda", sliding_window=150)
     values, seen_by = assert_same_numbers(got, want)
     assert 0 < values and 30 < seen_by < len(rows)
+
+
+def test_scales_of_a_bf16_cache():
+    """Scales are those of fp8 caches; a bf16 one holds its values as they are."""
+    s = prefix_inputs(8, 2, 64, 16, ODD, [200, 129])
+    want = prefix_call(ATTEND, s, "cuda")
+    assert torch.equal(prefix_call(ATTEND, {**s, "scales": (0.5, 0.25)}, "cuda"), want)
+    s = store_inputs(40, 4, 2, 64, 64, 16)
+    for got, want in zip(call(STORE, s, "cuda", change=dict(k_scale=0.5, v_scale=0.25)),
+                         call(STORE, s, "cuda")):
+        assert torch.equal(got, want)
