@@ -307,7 +307,7 @@ def shared_prefix_attention_decode(
     row of length 0 gives zeros, one longer than its table ends with it. Lengths and
     groups are read on the device only, so that a captured call follows them. Pages
     outside the cache are read as its nearest one. Scales are those of fp8 caches; a bf16
-    one holds its values as they are.
+    one holds its values as they are. A cache of no pages gives zeros.
     At most 4096 rows, 256 groups and 16 query heads a key/value head of 64 or 128.
     There is no gradient: a q that requires one is refused."""
     block_tables, seq_lens, prefix_group, prefix_lens = (

@@ -256,6 +256,8 @@ def shared_prefix_attention_decode(
     B, Hq, D = q.shape
     Hk, block_size = k_cache.shape[1:3]
     out = torch.zeros_like(q)
+    if k_cache.shape[0] == 0:
+        return out
     if k_cache.dtype != torch.float8_e4m3fn:  # scales are those of fp8 caches
         k_scale = v_scale = 1.0
     first = {}

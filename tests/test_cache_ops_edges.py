@@ -74,3 +74,10 @@ def test_scales_of_a_bf16_cache():
     for got, want in zip(call(STORE, s, change=dict(k_scale=0.5, v_scale=0.25)),
                          call(STORE, s)):
         assert torch.equal(got, want)
+
+
+def test_no_pages():
+    """A cache of no pages: zeros, as on the GPU."""
+    s = prefix_inputs(4, 2, 64, 16, ROWS, [20, 32])
+    s["kc"], s["vc"] = s["kc"][:0], s["vc"][:0]
+    assert (prefix_call(ATTEND, s, "cpu") == 0).all()
