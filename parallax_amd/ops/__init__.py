@@ -155,8 +155,8 @@ def qk_norm_rope_and_cache(
     are. One launch in place of the copies, norms and rope_and_cache().
 
     A slot below 0 or past the cache stores nothing (rows that pad a batch); a position
-    outside the table makes NaN; two rows of one slot leave either's values. There is no
-    gradient: inputs that require one are refused."""
+    outside the table makes NaN; two rows of one slot leave either's values. At most 2^20
+    heads. There is no gradient: inputs that require one are refused."""
     if positions.dtype is not torch.int32:
         positions = positions.to(torch.int32)
     if slot_mapping.dtype is not torch.int64:

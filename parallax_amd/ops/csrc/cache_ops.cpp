@@ -7,6 +7,7 @@
 
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <torch/extension.h>
 
 #include <hip/hip_runtime.h>
@@ -101,6 +102,7 @@ Tensor qk_norm_rope_and_cache(Tensor q, Tensor k, Tensor v, Tensor q_weight,
   TORCH_CHECK(v.sizes() == k.sizes(), "v must have k's sizes");
   TORCH_CHECK(Hq >= 1 && Hk >= 1 && D >= 1 && D <= 1024,
               "heads of 1 to 1024 values, one at least");
+  TORCH_CHECK(Hq + 2 * Hk <= 1 << 20, "at most 2^20 heads");
   check_list(q_weight, at::kBFloat16, D, "q_weight");
   check_list(k_weight, at::kBFloat16, D, "k_weight");
   check_cache(k_cache, v_cache, Hk, D);
@@ -143,6 +145,7 @@ Tensor qk_norm_rope_and_cache(Tensor q, Tensor k, Tensor v, Tensor q_weight,
   a.inv_k = (float)(1.0 / k_scale), a.inv_v = (float)(1.0 / v_scale);
   launch_head_norm_store(&a, neox, k_cache.scalar_type() == at::kFloat8_e4m3fn,
                          stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return out;
 }
 
@@ -234,5 +237,6 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   a.s_info = (int2*)take(B * 2);
   a.has = (int*)take(B);
   launch_shared_prefix(&a, fp8, stream());
+  C10_HIP_KERNEL_LAUNCH_CHECK();
   return out;
 }

@@ -312,15 +312,10 @@ __global__ __launch_bounds__(256) void head_norm_store16_kernel(const HeadNormSt
   }
 }
 
-extern "C" void launch_head_norm_store(const HeadNormStore* a, bool neox, bool fp8,
-                                       hipStream_t stream) {
-  const uintptr_t at = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v |
-                       (uintptr_t)a->q_w | (uintptr_t)a->k_w | (uintptr_t)a->out |
-                       (uintptr_t)a->k_cache | (uintptr_t)a->v_cache |
-                       (uintptr_t)a->cos_sin;
-  const int64_t strides =
-      a->q_row | a->q_head | a->k_row | a->k_head | a->v_row | a->v_head;
-  if (at % 16 || strides % 8 || a->D % 16 || a->rot % 16 || a->D > 512) {
+// many: as prompts are; vectors: everything lies as vectors need it
+static void launch_portion(const HeadNormStore* a, bool neox, bool fp8, bool many,
+                           bool vectors, hipStream_t stream) {
+  if (!vectors) {
     const int64_t items = (int64_t)a->T * (a->Hq + 2 * a->Hk);
     const dim3 grid((unsigned)((items + 3) / 4));
     auto run = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(*a); };
@@ -330,11 +325,6 @@ extern "C" void launch_head_norm_store(const HeadNormStore* a, bool neox, bool f
              : run(head_norm_store_kernel<false, false>);
     return;
   }
-  // Runs of slots and two heads a lane for prompts, a token's eight values a thread for
-  // decode. us without / with, 32 and 8 heads of 128 in bf16, two prompts: 256 tokens 5.6
-  // / 5.5, 512 8.4 / 5.6, 2,048 21 / 11.2, 8,192 84 / 38.5 (one head a lane 40.4, four
-  // 39.8); 96 and 256 requests of a slot each 4.1 / 12.3 and 6.9 / 14.8.
-  const bool many = a->T >= 512;
   const int64_t eights = (int64_t)a->Hk * (a->D / 8);
   const int64_t v_blocks =
       many ? (int64_t)ceil_div(a->T, 64) * (((eights + 15) / 16 + 1) / 2)
@@ -361,4 +351,31 @@ extern "C" void launch_head_norm_store(const HeadNormStore* a, bool neox, bool f
   else if (a->D <= 128) width(std::integral_constant<int, 8>{});
   else if (a->D <= 256) width(std::integral_constant<int, 16>{});
   else width(std::integral_constant<int, 32>{});
+}
+
+extern "C" void launch_head_norm_store(const HeadNormStore* a, bool neox, bool fp8,
+                                       hipStream_t stream) {
+  const uintptr_t at = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v |
+                       (uintptr_t)a->q_w | (uintptr_t)a->k_w | (uintptr_t)a->out |
+                       (uintptr_t)a->k_cache | (uintptr_t)a->v_cache |
+                       (uintptr_t)a->cos_sin;
+  const int64_t strides =
+      a->q_row | a->q_head | a->k_row | a->k_head | a->v_row | a->v_head;
+  const bool vectors = !(at % 16 || strides % 8 || a->D % 16 || a->rot % 16 || a->D > 512);
+  // Runs of slots and two heads a lane for prompts, a token's eight values a thread for
+  // decode. us without / with, 32 and 8 heads of 128 in bf16, two prompts: 256 tokens 5.6
+  // / 5.5, 512 8.4 / 5.6, 2,048 21 / 11.2, 8,192 84 / 38.5 (one head a lane 40.4, four
+  // 39.8); 96 and 256 requests of a slot each 4.1 / 12.3 and 6.9 / 14.8.
+  const bool many = a->T >= 512;
+  // A launch has less than 2^32 threads, 2^24 workgroups: of n tokens' heads either form
+  // has half of that at most, for up to 2^20 heads.
+  const int n = (1 << 25) / (a->Hq + 2 * a->Hk);
+  for (int64_t t0 = 0; t0 < a->T; t0 += n) {
+    HeadNormStore b = *a;
+    b.T = (int)(a->T - t0 < n ? a->T - t0 : n);
+    b.out += t0 * a->Hq * a->D;
+    b.q += t0 * a->q_row, b.k += t0 * a->k_row, b.v += t0 * a->v_row;
+    b.positions += t0, b.slots += t0;
+    launch_portion(&b, neox, fp8, many, vectors, stream);
+  }
 }

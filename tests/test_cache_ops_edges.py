@@ -81,3 +81,11 @@ def test_no_pages():
     s = prefix_inputs(4, 2, 64, 16, ROWS, [20, 32])
     s["kc"], s["vc"] = s["kc"][:0], s["vc"][:0]
     assert (prefix_call(ATTEND, s, "cpu") == 0).all()
+
+
+@EXT
+def test_too_many_heads_refused():
+    s = store_inputs(1, 1, 1, 2, 2, 16)
+    q = torch.zeros(1, (1 << 20) - 1, 2, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="2\\^20 heads"):
+        call(ops._require_ext("test").qk_norm_rope_and_cache, s, change=dict(q=q))

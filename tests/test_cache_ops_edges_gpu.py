@@ -119,3 +119,32 @@ def test_scales_of_a_bf16_cache():
     for got, want in zip(call(STORE, s, "cuda", change=dict(k_scale=0.5, v_scale=0.25)),
                          call(STORE, s, "cuda")):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T,D,rot", [(1 << 25, 1, 0), (1 << 26, 16, 16)])
+def test_more_rows_than_a_launch_has(T, D, rot):
+    """Of one head: more than 2^26 waves of the form for any sizes, more than 2^24
+    workgroups of the other. The same as in portions."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    b = torch.bfloat16
+    q, k, v = (torch.randn(T, 1, D, generator=g, device="cuda", dtype=b) for _ in range(3))
+    qw, kw = (1 + torch.randn(2, D, generator=g, device="cuda")).to(b)
+    table = torch.randn(50, rot, generator=g, device="cuda")
+    pos = torch.randint(0, 50, (T,), generator=g, device="cuda", dtype=torch.int32)
+    slots = torch.randperm(T // 64, generator=g, device="cuda")[:, None] * 64 + torch.arange(
+        64, device="cuda")
+    slots = slots.view(-1)
+
+    def caches():
+        return (torch.zeros(T // 16, 1, 16, D, dtype=b, device="cuda"),
+                torch.zeros(T // 16, 1, D, 16, dtype=b, device="cuda"))
+
+    kc, vc = caches()
+    out = STORE(q, k, v, qw, kw, 1e-5, kc, vc, pos, table, slots)
+    kc2, vc2 = caches()
+    n = 1 << 22
+    for a in range(0, T, n):
+        at = slice(a, a + n)
+        part = STORE(q[at], k[at], v[at], qw, kw, 1e-5, kc2, vc2, pos[at], table, slots[at])
+        assert torch.equal(out[at], part)
+    assert torch.equal(kc, kc2) and torch.equal(vc, vc2) and bool((vc != 0).any())
