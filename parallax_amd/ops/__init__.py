@@ -53,6 +53,13 @@ def _require_ext(op_name: str):
     return ext
 
 
+def _as_int32(t: torch.Tensor) -> torch.Tensor:
+    """What lies outside of 32 bits becomes their end on its side, not another number."""
+    if t.dtype is torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
+    return t if t.dtype is torch.int32 else t.to(torch.int32)
+
+
 # -- normalization ------------------------------------------------------------
 
 
@@ -157,8 +164,7 @@ def qk_norm_rope_and_cache(
     A slot below 0 or past the cache stores nothing (rows that pad a batch); a position
     outside the table makes NaN; two rows of one slot leave either's values. At most 2^20
     heads. There is no gradient: inputs that require one are refused."""
-    if positions.dtype is not torch.int32:
-        positions = positions.to(torch.int32)
+    positions = _as_int32(positions)
     if slot_mapping.dtype is not torch.int64:
         slot_mapping = slot_mapping.to(torch.int64)
     if q.is_cuda:
@@ -311,8 +317,7 @@ def shared_prefix_attention_decode(
     At most 4096 rows, 256 groups and 16 query heads a key/value head of 64 or 128.
     There is no gradient: a q that requires one is refused."""
     block_tables, seq_lens, prefix_group, prefix_lens = (
-        t if t.dtype is torch.int32 else t.to(torch.int32)
-        for t in (block_tables, seq_lens, prefix_group, prefix_lens))
+        _as_int32(t) for t in (block_tables, seq_lens, prefix_group, prefix_lens))
     if sinks is not None:
         sinks = sinks.float()
     if q.is_cuda:

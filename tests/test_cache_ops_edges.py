@@ -89,3 +89,24 @@ def test_too_many_heads_refused():
     q = torch.zeros(1, (1 << 20) - 1, 2, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="2\\^20 heads"):
         call(ops._require_ext("test").qk_norm_rope_and_cache, s, change=dict(q=q))
+
+
+def test_wide_integers():
+    """Lengths, groups, pages and positions of 64 bits are what they say, not what is
+    left of them in 32."""
+    s = prefix_inputs(4, 2, 64, 16, [(0, 48), (0, 48), (1, 48), (2, 48)], [20, 30])
+    s["tables"] = s["tables"][:, :3].contiguous()
+    s["kc"], s["vc"] = (x.float().nan_to_num().bfloat16() for x in (s["kc"], s["vc"]))
+    want = prefix_call(ATTEND, s, "cpu")
+    wide = {**s, **{n: s[n].long() for n in ("lens", "group", "tables", "prefix")}}
+    wide["lens"][1] += 1 << 32
+    wide["group"][3] += (1 << 32) - 2       # not group 0
+    assert torch.equal(prefix_call(ATTEND, wide, "cpu"), want)
+    wide["tables"][0, 1] = 1 << 32          # the last page, not the first
+    s["tables"][0, 1] = s["kc"].shape[0] - 1
+    assert torch.equal(prefix_call(ATTEND, wide, "cpu"), prefix_call(ATTEND, s, "cpu"))
+    s = store_inputs(6, 4, 2, 64, 64, 16)
+    s["pos"] = s["pos"].long()
+    s["pos"][2] += 1 << 32
+    q, kc, vc = call(STORE, s)
+    assert q[2].isnan().all() and not q[:2].isnan().any() and not q[3:].isnan().any()

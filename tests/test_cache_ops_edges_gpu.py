@@ -148,3 +148,25 @@ def test_more_rows_than_a_launch_has(T, D, rot):
         part = STORE(q[at], k[at], v[at], qw, kw, 1e-5, kc2, vc2, pos[at], table, slots[at])
         assert torch.equal(out[at], part)
     assert torch.equal(kc, kc2) and torch.equal(vc, vc2) and bool((vc != 0).any())
+
+
+def test_wide_integers():
+    """Lengths, groups, pages and positions of 64 bits are what they say, not what is
+    left of them in 32."""
+    s = prefix_inputs(4, 2, 64, 16, [(0, 48), (0, 48), (1, 48), (2, 48)], [20, 30])
+    s["tables"] = s["tables"][:, :3].contiguous()
+    s["kc"], s["vc"] = (x.float().nan_to_num().bfloat16() for x in (s["kc"], s["vc"]))
+    want = prefix_call(ATTEND, s, "cuda")
+    wide = {**s, **{n: s[n].long() for n in ("lens", "group", "tables", "prefix")}}
+    wide["lens"][1] += 1 << 32
+    wide["group"][3] += (1 << 32) - 2       # not group 0
+    assert torch.equal(prefix_call(ATTEND, wide, "cuda"), want)
+    wide["tables"][0, 1] = 1 << 32          # the last page, not the first
+    s["tables"][0, 1] = s["kc"].shape[0] - 1
+    assert torch.equal(prefix_call(ATTEND, wide, "cuda"),
+                       prefix_call(ATTEND, s, "cuda"))
+    s = store_inputs(6, 4, 2, 64, 64, 16)
+    pos = s["pos"].long()
+    pos[2] += 1 << 32
+    q, kc, vc = call(STORE, s, "cuda", change=dict(positions=pos.cuda()))
+    assert q[2].isnan().all() and not q[:2].isnan().any() and not q[3:].isnan().any()
