@@ -78,9 +78,10 @@ void check_no_grad(std::initializer_list<const Tensor*> tensors) {
     TORCH_CHECK(!t->requires_grad(), "there is no gradient: call it under no_grad");
 }
 
-float scale_of(double s, const char* name) {
-  TORCH_CHECK(std::isfinite(s) && s > 0, name, " must be above 0");
-  return (float)s;
+// of 32 bits, as the kernels take it and its inverse
+void check_scale(double s, const char* name) {
+  TORCH_CHECK(s > 0 && std::isfinite((float)s) && std::isfinite((float)(1.0 / s)), name,
+              " must be above 0, itself and its inverse within 32 bits");
 }
 
 Tensor from16(const Tensor& t) { return (uintptr_t)t.data_ptr() % 16 ? t.clone() : t; }
@@ -114,10 +115,11 @@ Tensor qk_norm_rope_and_cache(Tensor q, Tensor k, Tensor v, Tensor q_weight,
   const int64_t rot = cos_sin.size(1), P = cos_sin.size(0);
   TORCH_CHECK(rot % 2 == 0 && rot <= D && P <= INT_MAX && (P >= 1 || T == 0),
               "cos_sin must have a row a position, of an even width up to ", D);
-  TORCH_CHECK(eps >= 0, "eps must not be negative");
+  TORCH_CHECK(eps >= 0 && std::isfinite((float)eps),
+              "eps must not be negative, and within 32 bits");
   TORCH_CHECK(T * (Hq + 2 * Hk) <= INT_MAX && k_cache.size(2) <= INT_MAX, "too many rows");
-  scale_of(k_scale, "k_scale");
-  scale_of(v_scale, "v_scale");
+  check_scale(k_scale, "k_scale");
+  check_scale(v_scale, "v_scale");
   check_no_grad({&q, &k, &v, &q_weight, &k_weight});
   check_device(q, {&k, &v, &q_weight, &k_weight, &k_cache, &v_cache, &positions,
                    &cos_sin, &slot_mapping});
@@ -182,11 +184,14 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
                   B * (max_blocks * BS / 32 + 1) < INT_MAX / 2 &&
                   Hk * BS * D <= INT_MAX && Hq <= 65535,
               "too many tokens or heads");
-  TORCH_CHECK(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0,
-              "scale and softcap must be finite, softcap not negative");
+  TORCH_CHECK(std::isfinite((float)scale) && std::isfinite(softcap) && softcap >= 0,
+              "scale and softcap must be finite, softcap not negative, scale within 32 bits");
   if (sinks) check_list(*sinks, at::kFloat, Hq, "sinks");
-  scale_of(k_scale, "k_scale");
-  scale_of(v_scale, "v_scale");
+  check_scale(k_scale, "k_scale");
+  check_scale(v_scale, "v_scale");
+  const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(!fp8 || std::isfinite((float)(scale * k_scale)),
+              "scale times k_scale must be within 32 bits");
   check_no_grad({&q});
   check_device(q, {&k_cache, &v_cache, &block_tables, &seq_lens, &prefix_group,
                    &prefix_lens});
@@ -199,7 +204,6 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   v_cache = from16(v_cache);
   if ((uintptr_t)q.data_ptr() % 16 || q.stride(0) % 8) q = q.clone(at::MemoryFormat::Contiguous);
   if (max_blocks == 0 || k_cache.size(0) == 0) return out.zero_();
-  const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
   SharedPrefix a = {};
   a.out = (uint16_t*)out.data_ptr();
   a.q = (const uint16_t*)q.data_ptr();

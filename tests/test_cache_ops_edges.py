@@ -110,3 +110,28 @@ def test_wide_integers():
     s["pos"][2] += 1 << 32
     q, kc, vc = call(STORE, s)
     assert q[2].isnan().all() and not q[:2].isnan().any() and not q[3:].isnan().any()
+
+
+@EXT
+@pytest.mark.parametrize("change", [
+    dict(scale=1e39), dict(k_scale=1e39), dict(v_scale=1e39), dict(k_scale=1e-46),
+    dict(v_scale=1e-46), dict(k_scale=float("nan")), dict(softcap=float("nan")),
+])
+def test_beyond_fp32_refused(change):
+    """What fp32 cannot hold."""
+    s = prefix_inputs(4, 2, 64, 16, [(0, 40), (0, 21), (-1, 17)], [20])
+    with pytest.raises(RuntimeError) as e:
+        ops._require_ext("test").shared_prefix_attention_decode(*arguments(s, change))
+    assert "must be on GPU" not in str(e.value)
+
+
+@EXT
+@pytest.mark.parametrize("change", [
+    dict(k_scale=1e39), dict(v_scale=1e39), dict(k_scale=1e-46), dict(v_scale=1e-46),
+    dict(k_scale=1e-40), dict(eps=float("inf")), dict(eps=1e39), dict(eps=float("nan")),
+])
+def test_store_beyond_fp32_refused(change):
+    s = store_inputs(5, 4, 2, 64, 64, 16)
+    with pytest.raises(RuntimeError) as e:
+        call(ops._require_ext("test").qk_norm_rope_and_cache, s, change=change)
+    assert "must be on GPU" not in str(e.value)
