@@ -315,7 +315,7 @@ def shared_prefix_attention_decode(
     outside the cache are read as its nearest one. Scales are those of fp8 caches; a bf16
     one holds its values as they are. A cache of no pages gives zeros.
     At most 4096 rows, 256 groups and 16 query heads a key/value head of 64 or 128.
-    There is no gradient: a q that requires one is refused."""
+    There is no gradient: inputs that require one are refused."""
     block_tables, seq_lens, prefix_group, prefix_lens = (
         _as_int32(t) for t in (block_tables, seq_lens, prefix_group, prefix_lens))
     if sinks is not None:

@@ -120,7 +120,7 @@ Tensor qk_norm_rope_and_cache(Tensor q, Tensor k, Tensor v, Tensor q_weight,
   TORCH_CHECK(T * (Hq + 2 * Hk) <= INT_MAX && k_cache.size(2) <= INT_MAX, "too many rows");
   check_scale(k_scale, "k_scale");
   check_scale(v_scale, "v_scale");
-  check_no_grad({&q, &k, &v, &q_weight, &k_weight});
+  check_no_grad({&q, &k, &v, &q_weight, &k_weight, &k_cache, &v_cache, &cos_sin});
   check_device(q, {&k, &v, &q_weight, &k_weight, &k_cache, &v_cache, &positions,
                    &cos_sin, &slot_mapping});
   const c10::DeviceGuard guard(q.device());
@@ -192,7 +192,8 @@ Tensor shared_prefix_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache,
   const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
   TORCH_CHECK(!fp8 || std::isfinite((float)(scale * k_scale)),
               "scale times k_scale must be within 32 bits");
-  check_no_grad({&q});
+  check_no_grad({&q, &k_cache, &v_cache});
+  if (sinks) check_no_grad({&*sinks});
   check_device(q, {&k_cache, &v_cache, &block_tables, &seq_lens, &prefix_group,
                    &prefix_lens});
   if (sinks) check_device(q, {&*sinks});

@@ -132,7 +132,8 @@ def qk_norm_rope_and_cache(
     if rot % 2 or rot > D or k.shape != v.shape or k.shape[0] != T or k.shape[2] != D:
         raise RuntimeError("q, k, v and cos_sin do not fit each other")
     if torch.is_grad_enabled() and any(
-            t.requires_grad for t in (q, k, v, q_weight, k_weight)):
+            t.requires_grad
+            for t in (q, k, v, q_weight, k_weight, k_cache, v_cache, cos_sin)):
         raise RuntimeError("there is no gradient: call it under no_grad")
     known = (positions >= 0) & (positions < P)
     cs = cos_sin[positions.long().clamp(0, max(P - 1, 0))].masked_fill(
@@ -251,7 +252,8 @@ def shared_prefix_attention_decode(
 ) -> torch.Tensor:
     """A row's tokens before its group's prefix through the pages of the group's first
     row, the others through its own."""
-    if torch.is_grad_enabled() and q.requires_grad:
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (q, k_cache, v_cache, sinks)):
         raise RuntimeError("there is no gradient: call it under no_grad")
     B, Hq, D = q.shape
     Hk, block_size = k_cache.shape[1:3]

@@ -135,3 +135,30 @@ def test_store_beyond_fp32_refused(change):
     with pytest.raises(RuntimeError) as e:
         call(ops._require_ext("test").qk_norm_rope_and_cache, s, change=change)
     assert "must be on GPU" not in str(e.value)
+
+
+@EXT
+@pytest.mark.parametrize("native", [False, True])
+@pytest.mark.parametrize("name", ["k_cache", "v_cache", "sinks"])
+def test_no_gradient_of_what_is_read(name, native):
+    s = prefix_inputs(4, 2, 64, 16, [(0, 40), (0, 21), (-1, 17)], [20])
+    fn = (ops._require_ext("test") if native else ops).shared_prefix_attention_decode
+    leaf = dict(k_cache=s["kc"], v_cache=s["vc"], sinks=torch.zeros(4))[name]
+    change = {name: leaf.clone().requires_grad_()}
+    with pytest.raises(RuntimeError, match="no gradient"):
+        fn(*arguments(s, change))
+    with torch.no_grad():
+        if not native:
+            fn(*arguments(s, change))
+
+
+@EXT
+@pytest.mark.parametrize("native", [False, True])
+@pytest.mark.parametrize("name", ["k_cache", "v_cache", "cos_sin"])
+def test_store_no_gradient_of_caches_and_table(name, native):
+    s = store_inputs(5, 4, 2, 64, 64, 16)
+    _, _, _, a = store_views(s, "cpu")
+    leaf = dict(k_cache=a["kc"], v_cache=a["vc"], cos_sin=a["table"])[name]
+    fn = ops._require_ext("test").qk_norm_rope_and_cache if native else STORE
+    with pytest.raises(RuntimeError, match="no gradient"):
+        call(fn, s, change={name: leaf.clone().requires_grad_()})
