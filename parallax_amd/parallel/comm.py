@@ -131,6 +131,14 @@ class CommContext:
                 w, b = self._send_slots[key]
                 self._send_slots[key] = (None, b)
 
+    def gather_objects(self, obj) -> list:
+        """What each rank has, on every rank, for start-up: not for the step path."""
+        if self.world_size == 1 or not dist.is_initialized():
+            return [obj]
+        out = [None] * self.world_size
+        dist.all_gather_object(out, obj)
+        return out
+
     def barrier(self) -> None:
         if dist.is_initialized():
             dist.barrier()

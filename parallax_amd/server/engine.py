@@ -280,8 +280,7 @@ class Engine:
         if args.fused_head_norms:
             self._fuse_head_norms()
         self.shared_prefixes = None
-        if args.shared_prefix_attention:
-            self._check_shared_prefixes()
+        if args.shared_prefix_attention and self._shares_prefixes():
             self.shared_prefixes = SharedPrefixes(self.kv_cache.spec)
         self.graph_runner = None
         if args.enable_graphs and self.device.type == "cuda" \
@@ -325,9 +324,12 @@ class Engine:
                 and type(m).forward is LlamaAttention.forward
                 and type(m).attend is LlamaAttention.attend]
 
+    # Stages hold different layers: what one of them lacks is known to all before any is
+    # refused, or else the others would wait for it.
+
     def _fuse_head_norms(self) -> None:
         modules = [m for m in self._attentions() if m.qk_norm and not m.qk_norm_full]
-        if not modules:
+        if not any(self.comm.gather_objects(len(modules))):
             raise ValueError(
                 f"fused_head_norms: {self.cfg.architecture} has no norms of single heads")
         if self.device.type == "cuda" and self.args.dtype != torch.bfloat16:
@@ -335,24 +337,32 @@ class Engine:
         for m in modules:
             m.fused_head_norms = True
 
-    def _check_shared_prefixes(self) -> None:
+    def _shares_prefixes(self) -> bool:
+        """Whether a layer of this stage does; refused if the model's cannot."""
         modules = self._attentions()
-        if not modules or self.is_mla or self.cfg.has_linear_layers or len(modules) < sum(
+        problems = self.comm.gather_objects(self._sharing_problem(modules))
+        for problem in problems:
+            if problem:
+                raise ValueError(f"shared_prefix_attention{problem}")
+        return any(m.sliding_window <= 0 for m in modules)
+
+    def _sharing_problem(self, modules: List[LlamaAttention]) -> Optional[str]:
+        cfg, args = self.cfg, self.args
+        if not modules or self.is_mla or cfg.has_linear_layers or len(modules) < sum(
                 isinstance(m, LlamaAttention) for m in self.model.modules()):
-            raise ValueError(f"shared_prefix_attention: {self.cfg.architecture} has "
-                             "layers without it")
-        if all(m.sliding_window > 0 for m in modules):
-            raise ValueError("shared_prefix_attention: all layers have windows")
-        if not self.args.enable_prefix_cache:
-            raise ValueError("shared_prefix_attention needs the prefix cache")
+            return f": {cfg.architecture} has layers without it"
+        if cfg.sliding_window > 0 and all(
+                cfg.layer_type(g) == "sliding_attention" for g in range(cfg.num_layers)):
+            return ": all layers have windows"
+        if not args.enable_prefix_cache:
+            return " needs the prefix cache"
         if self.device.type == "cuda" and (
-                self.args.dtype != torch.bfloat16
-                or self.args.block_size not in (16, 32, 64)
+                args.dtype != torch.bfloat16 or args.block_size not in (16, 32, 64)
                 or any(m.head_dim not in (64, 128)
                        or m.num_heads > 16 * m.num_kv_heads for m in modules)):
-            raise ValueError(
-                "shared_prefix_attention needs bfloat16, pages of 16, 32 or 64 tokens, "
-                "heads of 64 or 128 and at most 16 query heads a key/value head")
+            return (" needs bfloat16, pages of 16, 32 or 64 tokens, heads of 64 or 128 "
+                    "and at most 16 query heads a key/value head")
+        return None
 
     # -- public API (head rank) ----------------------------------------------------
 
