@@ -170,3 +170,16 @@ def test_wide_integers():
     pos[2] += 1 << 32
     q, kc, vc = call(STORE, s, "cuda", change=dict(positions=pos.cuda()))
     assert q[2].isnan().all() and not q[:2].isnan().any() and not q[3:].isnan().any()
+
+
+@pytest.mark.parametrize("sink", [90.0, 1e4, 3e38, INF])
+def test_sinks_that_take_all(sink):
+    """Of a row that one wave finishes, of rows that are joined: nothing is left."""
+    s = prefix_inputs(4, 2, 64, 16, ODD, [200, 129])
+    sinks = torch.tensor([sink, 0.0, -INF, sink])
+    for kw in (dict(), dict(sliding_window=40)):
+        got = prefix_call(ATTEND, s, "cuda", sinks=sinks.cuda(), **kw)
+        # the oracle's softmax of an infinite sink is no number
+        want = prefix_oracle(s, sinks=sinks.clamp(max=1e30), **kw)
+        assert_attended(got, want)
+        assert (got[:, [0, 3]].abs() < 1e-30).all()
