@@ -117,6 +117,14 @@ struct Cap {
   }
 };
 
+// A sum of weights at maximum m with that of a sink, whichever is larger at 1. The weights
+// go by the square of what is returned, which may lie below what an exponential gives.
+DEVINL float beside_sink(float sink, float m, float& l) {
+  const float g = __builtin_amdgcn_exp2f(0.5f * fminf(m - sink, 0.f));
+  l = l * g * g + __builtin_amdgcn_exp2f(fminf(sink - m, 0.f));
+  return g;
+}
+
 // n / g of n below 2^20, exactly: n + 1/2 is 1/32 at least from where a quotient changes
 DEVINL int over(int n, int g) {
   return (int)(((float)n + 0.5f) * __builtin_amdgcn_rcpf((float)g));
@@ -997,14 +1005,14 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       if (l15 < G) {
         const int h = hk * G + l15;
         if (!t0.grouped && from <= lo && tok + KT >= L) {  // all that it sees
-          l += __builtin_amdgcn_exp2f(sink - m);
-          const float f = a.v_scale / l;
+          const float g = beside_sink(sink, m, l);
+          const float f = a.v_scale * g / l;
           uint16_t* dst = a.out + ((int64_t)t0.row * a.Hq + h) * D + l4 * 4;
 #pragma unroll
           for (int t = 0; t < MT; ++t)
             *reinterpret_cast<uint2*>(dst + t * 16) =
-                make_uint2(pack_bf16(o[t][0] * f, o[t][1] * f),
-                           pack_bf16(o[t][2] * f, o[t][3] * f));
+                make_uint2(pack_bf16(o[t][0] * f * g, o[t][1] * f * g),
+                           pack_bf16(o[t][2] * f * g, o[t][3] * f * g));
         } else {
           const int64_t part = (int64_t)(wave + t0.row) * a.Hq + h;
 #pragma unroll
@@ -1195,8 +1203,10 @@ __global__ __launch_bounds__(256) void shared_prefix_join_kernel(const SharedPre
 #pragma unroll
     for (int k = 1; k < W; ++k) s += sums[k][lane % Q];
   }
-  if (a.sinks != nullptr) l += __builtin_amdgcn_exp2f(a.sinks[h] * kLog2e - M);
-  s *= a.v_scale / l;
+  float g = 1.f;
+  if (a.sinks != nullptr) g = beside_sink(a.sinks[h] * kLog2e, M, l);
+  s *= a.v_scale * g / l;
+  s *= g;
   if (grp == 0)
     *reinterpret_cast<uint2*>(out) =
         make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));

@@ -181,5 +181,8 @@ def test_sinks_that_take_all(sink):
         got = prefix_call(ATTEND, s, "cuda", sinks=sinks.cuda(), **kw)
         # the oracle's softmax of an infinite sink is no number
         want = prefix_oracle(s, sinks=sinks.clamp(max=1e30), **kw)
-        assert_attended(got, want)
+        # below 2^-126 bf16 goes in steps of 2^-133: beside what a weight is off by, a
+        # rounding is off by up to 2^-134, which no share of the value covers
+        x = got.cpu().double()
+        assert_attended(x - (x - want[0]).clamp(-(2.0 ** -134), 2.0 ** -134), want)
         assert (got[:, [0, 3]].abs() < 1e-30).all()
