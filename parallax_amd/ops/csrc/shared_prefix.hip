@@ -147,7 +147,7 @@ struct Lists {
   int* prefix;      // the groups' lengths
   int* count;       // rows of a group
   int* low;         // where the first window of a group's rows begins
-  int* rows;        // of an item tile; [SP_ITEMS]: its group's first row, then a key tile
+  int* rows;        // of an item tile; [SP_ITEMS]: its group's first row, then a flag
   int2* span;       // of the first SP_SPANS rows: where a row's own tokens begin and end
   int16_t* member;  // a row's group, -1: none
   int* units;       // a row's suffix tiles; here the tiles come to lie
@@ -261,6 +261,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   const Cap capped(a);
 
   int done = 0;
+  bool careful = false;  // a segment's second time, see part_numbers()
   while (todo > 0) {
     const int n_items = uniform(w.count[g]) * G;
     const int P = uniform(w.prefix[g]);
@@ -276,7 +277,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     const int r1 = uniform(over(min((tile + 1) * SP_ITEMS, n_items) - 1, G));
     __syncthreads();  // the buffers and the list are free
     if (wid == 0) {
-      if (lane == 0) w.rows[SP_ITEMS + 1] = -1;
+      if (lane == 0) w.rows[SP_ITEMS + 1] = 0;
       int rank = 0;
       for (int b0 = 0; b0 < a.B && rank <= r1; b0 += 64) {
         const bool is = b0 + lane < a.B && w.member[b0 + lane] == g;
@@ -306,15 +307,15 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     }
     lo_most = uniform(lo_most);
     const int lo_least = uniform(w.low[g]);
-    int lo_last = 0;  // of the tile's rows
-    if (a.window > 0) {
+    int lo_last = 0;  // of the tile's rows, if careful
+    if (careful) {
       for (int i = lane; i <= r1 - r0; i += 64)
         lo_last = max(lo_last, window_start(a, length(a, w.rows[i])));
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1)
-        lo_last = max(lo_last, __shfl_xor(lo_last, o, WAVE_SIZE));
+      for (int i = 1; i < 64; i <<= 1)
+        lo_last = max(lo_last, __shfl_xor(lo_last, i, WAVE_SIZE));
+      lo_last = uniform(lo_last);
     }
-    lo_last = uniform(lo_last);
     const int part0 = apart ? run : run + tile0 + tile;
 
     if (k0 == kb && half == 0 && on)
@@ -451,20 +452,11 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       }
     };
 
-    // What one item sees and another's window hides must stay, and the other's weight 0
-    // times NaN or infinity would be NaN. A tile that has such values loses them here, and
-    // the items that see them get them as they are, behind their rescaling.
-    auto part_numbers = [&](int base, int tag, uint16_t* Vl) INL {
-      u32x4v* const mine = reinterpret_cast<u32x4v*>(Vl + wid * GROUP);
-      int* const found = w.rows + SP_ITEMS + 1;
-      uint32_t any = 0;
-#pragma unroll 1
-      for (int i = lane; i < GROUP / 8; i += 64)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) any |= (mine[i][j] & 0x7f807f80u) + 0x00800080u;
-      if ((any & 0x80008000u) != 0) *found = tag;
-      __syncthreads();
-      if (*found != tag) return;
+    // What one item sees and another's window hides stays in the product, and the other's
+    // weight 0 times NaN or infinity is NaN. Where that shows in a segment's sums it is gone
+    // through again, carefully: a tile that has such values loses them here, and the items
+    // that see them get them as they are, behind their rescaling.
+    auto part_numbers = [&](int base, uint16_t* Vl) INL {
       raise();
 #pragma unroll 1
       for (int tok = 0; tok < SP_KT; ++tok) {
@@ -483,6 +475,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
           }
       }
       __syncthreads();
+      u32x4v* const mine = reinterpret_cast<u32x4v*>(Vl + wid * GROUP);
 #pragma unroll 1
       for (int i = lane; i < GROUP / 8; i += 64) {
         u32x4v f = mine[i];
@@ -524,9 +517,8 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
         clean((kt - 1) * SP_KT, Vl);
         __syncthreads();
       }
-      const int prev = (kt - 1) * SP_KT;
-      if (!first && prev < lo_last && prev + SP_KT > lo_least)
-        part_numbers(prev, kt, Vl);
+      if (!first && (kt - 1) * SP_KT < lo_last && kt * SP_KT > lo_least)
+        part_numbers((kt - 1) * SP_KT, Vl);
       // operands are read AHEAD products early here too
       constexpr int AHEAD = 4;
       bf16x8v fr[AHEAD];
@@ -649,8 +641,10 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       }
     };
 
-    // the same for all waves where a turn has more barriers than one
-    const int whole = max(k0 + 1, (lo_last + SP_KT - 1) / SP_KT + 1);
+    // careful: the same turns for all waves, which have more barriers than one
+    const int whole = careful ? max(k0 + 1, (lo_last + SP_KT - 1) / SP_KT + 1)
+                              : max(max(k0 + 1, (lo_least + SP_KT - 1) / SP_KT + 1),
+                                    (lo_most + SP_KT - 1) / SP_KT);
     const int cut = wave_on && a.softcap <= 0.f ? min(k1, P / SP_KT) : 0;
 
     // The first turn's K, and behind it what that turn would ask for: the buffers are
@@ -695,6 +689,19 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
         }
       cut_turn(kt, odd);
     }
+    if (a.window > 0 && !careful) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          any |= (__float_as_uint(o[t][e]) & 0x7f800000u) + 0x00800000u;
+      if (any >> 31) w.rows[SP_ITEMS + 1] = 1;
+      __syncthreads();
+      careful = uniform(w.rows[SP_ITEMS + 1]);
+      if (careful) continue;
+    }
+    careful = false;
 
     l = over_halves(l, [](float x, float y) { return x + y; });
     if (on) {

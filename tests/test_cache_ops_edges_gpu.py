@@ -186,3 +186,19 @@ def test_sinks_that_take_all(sink):
         x = got.cpu().double()
         assert_attended(x - (x - want[0]).clamp(-(2.0 ** -134), 2.0 ** -134), want)
         assert (got[:, [0, 3]].abs() < 1e-30).all()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=30.0), dict(scale=-0.1)])
+@pytest.mark.parametrize("Hq,Hk,D,fp8", [
+    (8, 1, 128, False), (8, 2, 128, True), (2, 2, 64, False), (16, 1, 64, True)])
+def test_long_windows_over_no_numbers(Hq, Hk, D, fp8, kw):
+    """Windows that begin in other tiles for other waves, tiles that all see whole behind
+    them, two groups of which one has no such values, none that any row sees."""
+    rows = [(i % 2, 3000 + 20 * i) for i in range(60)]
+    s = prefix_inputs(Hq, Hk, D, 32, rows, [3000, 1500], fp8, seed=D)
+    for token in (300, 500, 2000):
+        put_value(s, 0, token, Hk - 1, 7, NAN)
+    put_value(s, 0, 90, 0, 9, NAN)  # hidden from all
+    got = prefix_call(ATTEND, s, "cuda", sliding_window=2900, **kw)
+    values, seen_by = assert_same_numbers(got, prefix_oracle(s, sliding_window=2900, **kw))
+    assert values == seen_by * (Hq // Hk) and seen_by == 30
