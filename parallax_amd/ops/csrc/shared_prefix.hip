@@ -95,11 +95,12 @@ DEVINL int page_at(const SharedPrefix& a, int entry) {
   return min(max(entry, 0), a.num_pages - 1);
 }
 
-// log2(e) cap tanh(y / cap) of a product s, whose score is y: y2 = 2 log2(e) y / cap,
-// flat = log2(e) y. From |y| = cap / 4 on by the exponential, off by some 2^-22 of the cap;
-// below, where that would be more than a weight may be off by, by tanh's series, the next
-// term of which is 2^-26 of the result. What it multiplies is y itself, so that caps far
-// above the scores leave them as they are.
+// log2(e) cap tanh(y / cap) of a product s, whose score is y, by the exponential of
+// 2 y / cap: off by some 2^-22 of the cap, 2^-15 of a weight at a cap of 64, which is less
+// than products in fp32 are off by. HIGH: of caps above that, below a quarter of them, by
+// tanh's series, the next term of which is 2^-26 of the result: what it multiplies is y
+// itself, so that caps far above the scores leave them as they are.
+template <bool HIGH>
 struct Cap {
   float flat, twice, cap;  // log2(e) |scale|, 2 log2(e) |scale| / cap, log2(e) cap
   DEVINL explicit Cap(const SharedPrefix& a)
@@ -107,12 +108,14 @@ struct Cap {
         twice(2.f * kLog2e * fabsf(a.scale) / fmaxf(a.softcap, 1e-30f)),
         cap(kLog2e * a.softcap) {}
   DEVINL float operator()(float s) const {
-    constexpr float t = 0.25f / (kLog2e * kLog2e);  // of y2^2: x^2
-    const float y2 = s * twice, x2 = y2 * y2 * t;
+    const float y2 = s * twice;
     const float e = __builtin_amdgcn_exp2f(y2);
-    const float bent = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e));
+    float bent = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e));
+    if constexpr (!HIGH) return bent;
+    const float x2 = y2 * y2 * (0.25f / (kLog2e * kLog2e));  // (y / cap)^2
     const float p = fmaf(fmaf(fmaf(fmaf(62.f / 2835, x2, -17.f / 315), x2, 2.f / 15), x2,
                               -1.f / 3), x2, 1.f);
+    asm volatile("" : "+v"(bent));  // both and a choice: a branch a score takes registers
     return x2 < 0.0625f ? s * flat * p : bent;
   }
 };
@@ -178,7 +181,7 @@ struct Lists {
 
 // ---- prefixes ----------------------------------------------------------------------
 
-template <int D, bool FP8>
+template <int D, bool FP8, bool HIGH>
 DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const int hk,
                         const int run, const int total, int per, const bool apart) {
   constexpr int KCH = D / 8;            // 16-byte chunks of a K row
@@ -258,7 +261,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
   };
   // above 0 also for a scale of 0: hidden scores are multiplied by it too
   const float c = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1e-20f);
-  const Cap capped(a);
+  const Cap<HIGH> capped(a);
 
   int done = 0;
   bool careful = false;  // a segment's second time, see part_numbers()
@@ -736,7 +739,7 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
 
 // ---- suffixes ----------------------------------------------------------------------
 
-template <int D, bool FP8>
+template <int D, bool FP8, bool HIGH>
 DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const int hk,
                         const int run, const int total, const int runs) {
   constexpr int KT = SP_UNIT;
@@ -796,7 +799,7 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
       FP8 ? lds_at(Vt) + l15 * VB + ((l4 >> 1) ^ swz_v<FP8>(l15)) * 16 + (l4 & 1) * 8
           : lds_at(Vt) + l15 * VB + (l4 ^ swz_v<FP8>(l15)) * 16;
   const float c = a.softcap > 0.f ? 1.f : fmaxf(fabsf(a.scale) * kLog2e, 1e-20f);
-  const Cap capped(a);
+  const Cap<HIGH> capped(a);
 
   // Rows 64 at a time, one a lane: where its own tokens begin and end.
   int rows0 = -64, row_lo = 0, row_end = 0;
@@ -1042,7 +1045,7 @@ DEVINL void suffix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
 
 }  // namespace
 
-template <int D, bool FP8>
+template <int D, bool FP8, bool HIGH>
 __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_kernel(
     const SharedPrefix a) {
   __shared__ __attribute__((aligned(1024))) uint8_t S[lds_bytes(D)];
@@ -1130,9 +1133,9 @@ __global__ __launch_bounds__(SP_THREADS, D == 64 ? 3 : 2) void shared_prefix_ker
     p_runs = uniform(used);  // the others are for suffixes
   }
   if (run < p_runs)
-    prefix_role<D, FP8>(a, w, S, hk, run, p_total, per, apart);
+    prefix_role<D, FP8, HIGH>(a, w, S, hk, run, p_total, per, apart);
   else
-    suffix_role<D, FP8>(a, w, S, hk, run - p_runs, s_total, a.runs - p_runs);
+    suffix_role<D, FP8, HIGH>(a, w, S, hk, run - p_runs, s_total, a.runs - p_runs);
 }
 
 // Joins the parts of every row and query head, W waves each. A lane takes a part for
@@ -1191,7 +1194,9 @@ __global__ __launch_bounds__(256) void shared_prefix_join_kernel(const SharedPre
       for (int j = 0; j < AHEAD; ++j) {
         const int i = j0 + first + j * W * GROUPS;
         const float y = __shfl(w, min(i, n - 1), WAVE_SIZE);
-        if (i < n) s += x[j] * y;  // else a part again: infinity times 0 is no number
+        const f32x4v z = x[j] * y;  // past the end a part again, of infinities perhaps
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += i < n ? z[e] : 0.f;
       }
       if (j0 + AHEAD * W * GROUPS < n)
 #pragma unroll
@@ -1230,9 +1235,17 @@ extern "C" void shared_prefix_plan(int B, int N, int Hq, int Hk, int D, int* run
 extern "C" void launch_shared_prefix(const SharedPrefix* a, bool fp8, hipStream_t stream) {
   const dim3 grid(a->runs * a->Hk);
   auto run = [&](auto kernel) { kernel<<<grid, SP_THREADS, 0, stream>>>(*a); };
-  if (a->D == 128) fp8 ? run(shared_prefix_kernel<128, true>)
-                       : run(shared_prefix_kernel<128, false>);
-  else fp8 ? run(shared_prefix_kernel<64, true>) : run(shared_prefix_kernel<64, false>);
+  auto pick = [&](auto high) {
+    constexpr bool H = decltype(high)::value;
+    if (a->D == 128) fp8 ? run(shared_prefix_kernel<128, true, H>)
+                         : run(shared_prefix_kernel<128, false, H>);
+    else fp8 ? run(shared_prefix_kernel<64, true, H>)
+             : run(shared_prefix_kernel<64, false, H>);
+  };
+  // us by the exponential / the series: 256 rows over 8,000 103 / 117, 100 rows in five
+  // groups over 5,000 of 64 42 / 51, 64 over 60,000 of an fp8 cache 250 / 316.
+  if (a->softcap > 64.f) pick(std::true_type{});
+  else pick(std::false_type{});
   // Few rows: four waves each, which share its parts. One / four, us of the call: 8
   // rows of 32 heads over 100,000 tokens 96.6 / 91.2, 256 over 8,000 98.6 / 108.6, 128 rows
   // of 64 heads over 256 tokens 26.0 / 34.6.

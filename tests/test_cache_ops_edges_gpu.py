@@ -30,7 +30,7 @@ def test_store_without_pages(T, D, rot, head_gap):
     assert_stored(call(STORE, s, "cuda"), *store_oracle(s, True))
 
 
-CAPS = [1e3, 1e5, 1e8, 1e30, 3e38, 1e300]
+CAPS = [64.0, 64.1, 1e3, 1e5, 1e8, 1e30, 3e38, 1e300]
 
 
 @pytest.mark.parametrize("softcap", CAPS)

@@ -119,7 +119,7 @@ def test_products_are_waited_for(tmp_path):
         capture_output=True)
     kernels = _functions(out.read_text())
     assert sum(any("mfma" in op for op, _ in code)
-               for code, _ in kernels.values()) == 4
+               for code, _ in kernels.values()) == 8
     for name, (code, labels) in kernels.items():
         early = [(*map(lambda i: " ".join([code[i][0], ", ".join(code[i][1])]), (a, b)), n)
                  for a, b, n in _too_early(code, labels)]
