@@ -58,17 +58,17 @@ DEVINL void read8(u32x4v (&v)[8], uint32_t a, uint32_t b, uint32_t c, uint32_t d
                : "v"(a), "v"(b), "v"(c), "v"(d), "n"(OFF) : "memory");
 }
 DEVINL void read_rows(u32x4v (&v)[4], uint32_t a) {
-  asm volatile(RD "%0, %4\n\t" RD "%1, %4 offset:1024\n\t"
-               RD "%2, %4 offset:2048\n\t" RD "%3, %4 offset:3*1024\n\t"
+  asm volatile(RD "%0, %4\n\t" RD "%1, %4 offset:1*1024\n\t"
+               RD "%2, %4 offset:2*1024\n\t" RD "%3, %4 offset:3*1024\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
                : "v"(a) : "memory");
 }
 DEVINL void read_rows(u32x4v (&v)[8], uint32_t a) {
-  asm volatile(RD "%0, %8\n\t" RD "%1, %8 offset:1024\n\t"
-               RD "%2, %8 offset:2048\n\t" RD "%3, %8 offset:3*1024\n\t"
-               RD "%4, %8 offset:4096\n\t" RD "%5, %8 offset:5120\n\t"
-               RD "%6, %8 offset:6144\n\t" RD "%7, %8 offset:7168\n\t"
+  asm volatile(RD "%0, %8\n\t" RD "%1, %8 offset:1*1024\n\t"
+               RD "%2, %8 offset:2*1024\n\t" RD "%3, %8 offset:3*1024\n\t"
+               RD "%4, %8 offset:4*1024\n\t" RD "%5, %8 offset:5*1024\n\t"
+               RD "%6, %8 offset:6*1024\n\t" RD "%7, %8 offset:7*1024\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]),
                  "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
@@ -77,17 +77,17 @@ DEVINL void read_rows(u32x4v (&v)[8], uint32_t a) {
 #undef RD
 #define RD "ds_read_b64 "
 DEVINL void read_rows(u32x2v (&v)[4], uint32_t a) {
-  asm volatile(RD "%0, %4\n\t" RD "%1, %4 offset:512\n\t"
-               RD "%2, %4 offset:1024\n\t" RD "%3, %4 offset:1536\n\t"
+  asm volatile(RD "%0, %4\n\t" RD "%1, %4 offset:1*512\n\t"
+               RD "%2, %4 offset:2*512\n\t" RD "%3, %4 offset:3*512\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
                : "v"(a) : "memory");
 }
 DEVINL void read_rows(u32x2v (&v)[8], uint32_t a) {
-  asm volatile(RD "%0, %8\n\t" RD "%1, %8 offset:512\n\t"
-               RD "%2, %8 offset:1024\n\t" RD "%3, %8 offset:1536\n\t"
-               RD "%4, %8 offset:2048\n\t" RD "%5, %8 offset:2560\n\t"
-               RD "%6, %8 offset:3*1024\n\t" RD "%7, %8 offset:3584\n\t"
+  asm volatile(RD "%0, %8\n\t" RD "%1, %8 offset:1*512\n\t"
+               RD "%2, %8 offset:2*512\n\t" RD "%3, %8 offset:3*512\n\t"
+               RD "%4, %8 offset:4*512\n\t" RD "%5, %8 offset:5*512\n\t"
+               RD "%6, %8 offset:6*512\n\t" RD "%7, %8 offset:7*512\n\t"
                "s_waitcnt lgkmcnt(0)"
                : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]),
                  "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
