@@ -13,9 +13,10 @@
 // both are the caller's fault, and neither may read or write past a buffer.
 //
 // What bounds it: prompts memory, 8,192 tokens of 32 and 8 heads of 128 in bf16 (206 MB)
-// 38.5 us or 5.3 TB/s in a row of calls, 42 among calls on other tensors; into an fp8
+// 38.5 us or 5.3 TB/s in a row of calls, 43 among calls on other tensors; into an fp8
 // cache 36. Decode latency: one token 2.7 us, 96 4.1, 200 rows of 64 and 8 heads
-// into an fp8 cache 6.1. Copies, norms and rope_and_cache() apart: one token 6.9.
+// into an fp8 cache 6.1. Copies, norms and rope_and_cache() apart: one token 6.6, 8,192
+// 173, those 200 rows 24.7.
 
 #include <type_traits>
 
@@ -365,7 +366,9 @@ extern "C" void launch_head_norm_store(const HeadNormStore* a, bool neox, bool f
   // Runs of slots and two heads a lane for prompts, a token's eight values a thread for
   // decode. us without / with, 32 and 8 heads of 128 in bf16, two prompts: 256 tokens 5.6
   // / 5.5, 512 8.4 / 5.6, 2,048 21 / 11.2, 8,192 84 / 38.5 (one head a lane 40.4, four
-  // 39.8); 96 and 256 requests of a slot each 4.1 / 12.3 and 6.9 / 14.8.
+  // 39.8); 96 and 256 requests of a slot each 4.1 / 12.3 and 6.9 / 14.8. Requests of a slot
+  // each pay for the rule from 512 on, as it knows rows alone: 511 10.1, 512 17.1, 1,024
+  // 30.6, where the launches apart take 31.6, 31.3 and 53.4.
   const bool many = a->T >= 512;
   // A launch has less than 2^32 threads, 2^24 workgroups: of n tokens' heads either form
   // has half of that at most, for up to 2^20 heads.

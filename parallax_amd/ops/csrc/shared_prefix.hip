@@ -25,19 +25,21 @@
 // Lengths, groups and prefixes are read on the device, by every workgroup itself; the
 // grid depends on sizes alone.
 //
-// What bounds it, replayed in graphs, 32 query heads over 8 of 128 in bf16 unless said:
+// What bounds it, replayed in graphs on several cards, 32 query heads over 8 of 128 in bf16
+// unless said:
 // Long prefixes by the products with the softmax's instructions beside them, and by the
-// card's power: 64 rows, 64 heads over 8, 60,000 shared tokens 152 us, of which this
-// launch has 141, 890 TFLOP/s, where a product of 8192^3 reaches 1,213; at 1.9 GHz matrix
-// and vector units are busy 42% and 44% of the time, and neither the order of a turn nor
-// how far ahead operands are read moves it. Of an fp8 cache 149, 181 with up to 4,000 more
-// tokens a row. Suffixes by the stream of their keys and values: 8 rows over 100,000, where
-// the prefix is little more than a stream too, 91 us, 4.5 TB/s. Both together: 256 rows
-// over 8,000, up to 600 of their own, 98, of which the prefix alone is 57 and the rest
-// alone 89. Small batches by waits in a row, of lengths, lists, page numbers, a tile, and
-// by the second launch: 4 rows over 700 tokens, 14 heads over 2 of 64, 10.6; 16 rows over
-// 500, up to 300 of their own, 15, where paged_decode.hip starts with 6. The second
-// launch is 4 to 10 of each, 9 where it reads the 34 MB that 512 workgroups leave.
+// card's power: 64 rows, 64 heads over 8, 60,000 shared tokens 152 to 160 us, of which this
+// launch has 143 to 151, 830 to 880 TFLOP/s, where a product of 8192^3 reaches 1,213; at
+// 1.9 GHz matrix and vector units are busy 42% and 44% of the time, and neither the order of
+// a turn nor how far ahead operands are read moves it. Of an fp8 cache 149 to 155, 182 to
+// 189 with up to 4,000 more tokens a row. Under a softcap, whose turns are all of the kind
+// for any, 203 to 210 in bf16. Suffixes by the stream of their keys and values: 8 rows over
+// 100,000, where the prefix is little more than a stream too, 92 us, 4.5 TB/s. Both
+// together: 256 rows over 8,000, up to 600 of their own, 98, of which the prefix alone is 58
+// and the rest alone 91. Small batches by waits in a row, of lengths, lists, page numbers, a
+// tile, and by the second launch: 4 rows over 700 tokens, 14 heads over 2 of 64, 11.0; 16
+// rows over 500, up to 300 of their own, 15, where paged_decode.hip starts with 6. The
+// second launch is 4 to 10 of each, 10 where it reads the 34 MB that 512 workgroups leave.
 //
 // Keys and values of 16-bit caches go to LDS by buffer instructions: behind global ones
 // the compiler waits for all reads of LDS at once, 164 us where these took 151.
@@ -409,8 +411,8 @@ DEVINL void prefix_role(const SharedPrefix& a, const Lists& w, uint8_t* S, const
     };
     // Rescaled whenever a maximum moved, which 32 items have in three turns of four: the
     // largest weight is then 1, without error. Only at moves by more than 2^8, 64 rows
-    // over 60,000 tokens take 149 us for 157, but the error against 64 bits goes from 1.8e-3
-    // of the result, of which its own rounding has 1.6e-3, to 2.3e-3.
+    // over 60,000 tokens took 149 us for 157 on one card, but the error against 64 bits
+    // goes from 1.8e-3 of the result, of which its own rounding has 1.6e-3, to 2.3e-3.
     auto raise = [&]() INL {
       if (__any(mx > m)) {
         const float m2 = fmaxf(m, mx);

@@ -25,6 +25,8 @@ from .kv_cache import KVCacheSpec
 # 22.6, 28.0. Whole decode steps, four layers of 8B's sizes, ms: 64 requests behind 1,024
 # shared tokens (264 MB) 1.006 shared, 0.996 plain; 2,048 (528 MB) 1.008, 1.061; 128 behind
 # 4,000 (2 GB) 1.497, 1.850; 256 behind 8,000 (8.4 GB) 2.460, 3.984.
+# With fused_head_norms the plain form does not store in its launch, and the shared one
+# passes it sooner, by the first figures from some 128 MB on; one limit serves both.
 LEAST_BYTES = 384 << 20
 MAX_GROUPS = 32    # as many as a graph's buffers hold; those that save most are kept
 MAX_ROWS = 4096    # the kernel's own limit
