@@ -126,7 +126,7 @@ struct Cap {
 // go by the square of what is returned, which may lie below what an exponential gives.
 DEVINL float beside_sink(float sink, float m, float& l) {
   const float g = __builtin_amdgcn_exp2f(0.5f * fminf(m - sink, 0.f));
-  l = l * g * g + __builtin_amdgcn_exp2f(fminf(sink - m, 0.f));
+  l = l * g * g + (sink > m ? 1.f : __builtin_amdgcn_exp2f(sink - m));  // NaN stays
   return g;
 }
 

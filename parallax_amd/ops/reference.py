@@ -282,7 +282,7 @@ def shared_prefix_attention_decode(
             cap = min(max(softcap, 1e-30), 1e38)
             z = (cap * torch.tanh(z.double() / cap)).float()
         if sinks is not None:
-            z = torch.cat([z, sinks.float().unsqueeze(-1)], dim=-1)
+            z = torch.cat([z, sinks.float().clamp(max=3e38).unsqueeze(-1)], dim=-1)
         p = torch.softmax(z, dim=-1)[:, : len(tok)].view(Hk, Hq // Hk, -1)
         out[b] = torch.einsum("hgl,lhd->hgd", p, v).reshape(Hq, D).to(q.dtype)
     return out

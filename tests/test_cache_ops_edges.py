@@ -162,3 +162,12 @@ def test_store_no_gradient_of_caches_and_table(name, native):
     fn = ops._require_ext("test").qk_norm_rope_and_cache if native else STORE
     with pytest.raises(RuntimeError, match="no gradient"):
         call(fn, s, change={name: leaf.clone().requires_grad_()})
+
+
+def test_sinks_that_take_all():
+    s = prefix_inputs(4, 2, 64, 16, ROWS, [20, 32])
+    inf = float("inf")
+    got = prefix_call(ATTEND, s, "cpu", sinks=torch.tensor([inf, 0.0, -inf, 3e38]))
+    want, size = prefix_oracle(s, sinks=torch.tensor([1e30, 0.0, -inf, 1e30]))
+    assert_attended(got, (want, size), weights=0.0)
+    assert (got[:, [0, 3]] == 0).all()

@@ -202,3 +202,14 @@ def test_long_windows_over_no_numbers(Hq, Hk, D, fp8, kw):
     got = prefix_call(ATTEND, s, "cuda", sliding_window=2900, **kw)
     values, seen_by = assert_same_numbers(got, prefix_oracle(s, sliding_window=2900, **kw))
     assert values == seen_by * (Hq // Hk) and seen_by == 30
+
+
+def test_sinks_that_are_no_numbers():
+    """Their heads are none, of rows of one part and of many, the others as ever."""
+    s = prefix_inputs(4, 2, 64, 16, ODD, [200, 129])
+    sinks = torch.tensor([NAN, 0.5, NAN, -2.0])
+    got = prefix_call(ATTEND, s, "cuda", sinks=sinks.cuda())
+    want, size = prefix_oracle(s, sinks=sinks.nan_to_num())
+    some = s["lens"] > 0
+    assert got[some][:, [0, 2]].isnan().all() and (got[~some] == 0).all()
+    assert_attended(got[:, [1, 3]], (want[:, [1, 3]], size[:, [1, 3]]))
