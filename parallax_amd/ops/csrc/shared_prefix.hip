@@ -45,6 +45,7 @@
 // the compiler waits for all reads of LDS at once, 164 us where these took 151.
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <type_traits>
 
@@ -107,7 +108,7 @@ struct Cap {
   float flat, twice, cap;  // log2(e) |scale|, 2 log2(e) |scale| / cap, log2(e) cap
   DEVINL explicit Cap(const SharedPrefix& a)
       : flat(kLog2e * fabsf(a.scale)),
-        twice(2.f * kLog2e * fabsf(a.scale) / fmaxf(a.softcap, 1e-30f)),
+        twice(fminf(2.f * kLog2e * fabsf(a.scale) / fmaxf(a.softcap, 1e-30f), FLT_MAX)),
         cap(kLog2e * a.softcap) {}
   DEVINL float operator()(float s) const {
     const float y2 = s * twice;

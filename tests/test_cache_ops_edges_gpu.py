@@ -213,3 +213,12 @@ def test_sinks_that_are_no_numbers():
     some = s["lens"] > 0
     assert got[some][:, [0, 2]].isnan().all() and (got[~some] == 0).all()
     assert_attended(got[:, [1, 3]], (want[:, [1, 3]], size[:, [1, 3]]))
+
+
+@pytest.mark.parametrize("softcap", [1e-20, 30.0, 1e10])
+def test_large_scales(softcap):
+    """Scores of 0, and others that a scale takes past any cap."""
+    s = prefix_inputs(4, 2, 64, 16, ODD, [200, 129])
+    s["q"][::2] = 0
+    got = prefix_call(ATTEND, s, "cuda", scale=1e25, softcap=softcap)
+    assert_attended(got, prefix_oracle(s, scale=1e25, softcap=softcap))
